@@ -90,6 +90,18 @@ SIGNATURES = {
                               c_int, _VP, c_int, _VP, c_size_t, _VP]),
     "dc_kv_cache_fill": (c_int, [_VP, c_int, c_int, c_int, c_int, _VP, _VP]),
     "dc_copy2d": (c_int, [_VP, c_size_t, _VP, c_size_t, c_size_t, c_size_t, _VP]),
+    "dc_page_tables": (c_int, [_VP, _VP, c_int, c_int, _VP, c_int, _VP, _VP, _VP, c_int, _VP, c_int, c_int,
+                               _VP, _VP]),
+    "dc_kv4_pages_size": (c_int, [c_int, c_int, c_int, POINTER(c_size_t)]),
+    "dc_kv4_write": (c_int, [_VP, _VP, c_int, c_int, _VP, c_int, c_int, _VP, c_int, c_int, _VP, _VP, c_int,
+                             _VP]),
+    "dc_aft_decode4_workspace_size": (c_size_t, [c_int, c_int]),
+    "dc_aft_decode4": (c_int, [_VP, c_int, c_int, _VP, c_int, ctypes.c_longlong, _VP, c_int, c_int, _VP,
+                               c_int, c_int, c_int, c_int, _VP, c_int, _VP, c_int, _VP, c_size_t, _VP]),
+    "dc_logits_controls": (c_int, [_VP, c_int, _VP, c_int, c_int, c_int, c_int, _VP, c_int, _VP, c_int, _VP,
+                                   _VP, _VP, _VP, _VP, c_int, _VP, c_int, _VP]),
+    "dc_greedy_embed_rows": (c_int, [_VP, c_int, c_int, c_int, c_int, _VP, _VP, _VP, _VP, c_int, _VP, c_int,
+                                     _VP, _VP]),
     # the reference's handle ABI
     "create_tensor": (_VP, [c_int32, c_int32, _FP]),
     "destroy_tensor": (None, [_VP]),

@@ -197,7 +197,8 @@ int dc_device_status(void *stream, int *bits)
         DC_CUDA_TRY(cudaMemset(w, 0, sizeof(int)));
         return dc::fail(DC_ERR_DEVICE, "device status bits 0x%x (0x1-0x10: a bounded wait gave up; "
                         "0x20: token id out of range; 0x40: decode past capacity; "
-                        "0x80: AFT input outside the factorised range)", h);
+                        "0x80: AFT input outside the factorised range; 0x100: no page for a token; "
+                        "0x200: a slot or page outside the history's pool)", h);
     }
     return DC_OK;
 }

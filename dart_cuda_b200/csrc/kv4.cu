@@ -1,0 +1,485 @@
+// A paged k/v history held in 4 bits, and the AFT-full decode step over it.
+//
+// History: pages of page_size positions, each [D/W][page_size][5W/4] bytes
+// (W, the slab width, is the largest of 256, 128, 64, 32 that divides D).  The
+// record of a slab's W channels at one position holds, per 8 channels, 4
+// bytes of k codes and 4 of v codes (channel j in bits 4j..4j+3), then per
+// group of 32 channels four bf16: k step, k low, v step, v low.  A code c
+// stands for low + step * c: 5 bits a value instead of 32, and a lane's 8
+// channels are one 8-byte word.
+//
+// Quantisation of a group (k and v apart): low is the largest bf16 <= min x,
+// step the smallest bf16 >= (max x - low) / 15, so that 0..15 cover the group
+// whatever its offset, and code = floor((x - low) / step + 1/2), decided
+// exactly: x >= low + step (c + 1/2) holds in real numbers iff it holds
+// against that border rounded up to fp32 (x is an fp32 number).  |x - value|
+// <= step / 2.  A group with a value that is not finite (or above 1e38 in
+// magnitude) is stored with a NaN step: all its channels read as NaN.
+//
+// The decode step is dc_aft_decode's row t of AFT-full
+// (native/src/kernels/attention.cuh:6-40),
+//
+//   Z[b,c] = sigmoid(q[b,c]) * sum_{i<=t} e^{k_i[c] + w[t,i]} v_i[c] / sum_{i<=t} e^{k_i[c] + w[t,i]},
+//
+// with t = pos[b] of its own for every sequence and the rows found through a
+// block table.  The reference recomputes the whole context per token
+// (example/bin/shakespear4.dart:176-214) and keeps no history.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "dc_internal.h"
+#include "dc_ptx.cuh"
+
+namespace dc {
+namespace kv4 {
+
+constexpr float kBig = 1e38f;        // larger magnitudes count as not finite
+constexpr int DC_DEVERR_FULL = 0x40;  // a position past the capacity
+constexpr int DC_DEVERR_PAGE = 0x200; // a slot or page id outside the pool
+constexpr float kLog2e = 1.4426950408889634f;
+
+static int slab_width(int D)
+{
+    for (int w = 256; w >= 32; w /= 2)
+        if (D % w == 0) return w;
+    return 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float *p, float (&x)[8])
+{
+    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16 *p, float (&x)[8])
+{
+    const uint4 a = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[2 * j] = __uint_as_float(u[j] << 16);
+        x[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T *p, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float *p, const float (&x)[8])
+{
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16 *p, const float (&x)[8])
+{
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+        u[j] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// One group's quantisation by the 4 lanes (xor 1, 2) that hold its 32 values:
+// step and low (bf16 values, the same on the 4 lanes), this lane's 8 codes.
+// All 32 lanes of the warp take part.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, float &low)
+{
+    float mn = x[0], mx = x[0];
+    int bad = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        mn = fminf(mn, x[j]);
+        mx = fmaxf(mx, x[j]);
+        bad |= !(fabsf(x[j]) <= kBig);
+    }
+#pragma unroll
+    for (int o = 1; o <= 2; o *= 2) {
+        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    if (bad) {
+        step = __uint_as_float(0x7fff0000u);
+        low = 0.f;
+        return 0;
+    }
+    uint32_t cut = __float_as_uint(mn) & 0xffff0000u;  // towards zero
+    if (__uint_as_float(cut) > mn) cut += 0x10000u;
+    low = __uint_as_float(cut == 0x80000000u ? 0u : cut);  // -0 is stored as 0
+    const float up = __fdiv_ru(__fsub_ru(mx, low), 15.f);
+    step = __uint_as_float((__float_as_uint(up) + 0xffffu) & 0xffff0000u);
+    if (step == 0.f) {  // -0 - 0 among them
+        step = 0.f;
+        return 0;
+    }
+    uint32_t codes = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float c = fminf(fmaxf(floorf(__fdiv_rn(x[j] - low, step) + 0.5f), 0.f), 15.f);
+        // the estimate is within one of the code; the borders decide
+        if (c > 0.f && x[j] < __fmaf_ru(step, c - 0.5f, low))
+            c -= 1.f;
+        else if (c < 15.f && x[j] >= __fmaf_ru(step, c + 0.5f, low))
+            c += 1.f;
+        codes |= (uint32_t)c << (4 * j);
+    }
+    return codes;
+}
+
+__device__ __forceinline__ uint32_t pack_params(float step, float low)
+{
+    return (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+}
+
+// The 8 values that codes stand for.
+__device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (&x)[8])
+{
+    const float step = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
+}
+
+// Byte offset of the record of slab `slab` at slot (page, row).
+__device__ __forceinline__ size_t record(int page, int row, int slab, int nslab, int page_size, int W)
+{
+    return (((size_t)page * nslab + slab) * page_size + row) * (size_t)(W * 5 / 4);
+}
+
+struct Write {
+    const void *k, *v;
+    int64_t ld;
+    const int32_t *slots;
+    int n, D, W, page_size, n_pages;
+    uint8_t *pages;
+    void *vk, *vv;
+    int64_t ldv;
+    int *status;
+};
+
+// One lane per 8 channels of a row (k and v); rows with a negative slot are
+// left out.
+template <typename T>
+__global__ void __launch_bounds__(256) write_kernel(Write p)
+{
+    grid_dep_wait();  // programmatic dependent launch: inputs are ready
+    grid_dep_launch();
+    const int octs = p.D / 8;
+    const int64_t total = (int64_t)p.n * octs;  // a multiple of 4: groups stay within a warp
+    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+    const int64_t first = (int64_t)blockIdx.x * blockDim.x + (threadIdx.x & ~31);
+    for (int64_t base = first; base < total; base += stride) {
+        const int64_t at = base + (threadIdx.x & 31);
+        const bool in = at < total;
+        const int row = in ? (int)(at / octs) : 0;
+        const int ch = in ? (int)(at % octs) * 8 : 0;
+        const int slot = in ? p.slots[row] : -1;
+        const bool ok = slot >= 0 && slot < (int64_t)p.n_pages * p.page_size;
+        float k[8] = {}, v[8] = {};
+        if (ok) {
+            load8(static_cast<const T *>(p.k) + row * p.ld + ch, k);
+            load8(static_cast<const T *>(p.v) + row * p.ld + ch, v);
+        } else if (slot >= 0 && ch == 0) {
+            atomicOr(p.status, DC_DEVERR_PAGE);
+        }
+        float ks, kl, vs, vl;
+        const uint32_t kc = quantise8(k, ks, kl), vc = quantise8(v, vs, vl);
+        if (!ok) continue;
+        const uint32_t kp = pack_params(ks, kl), vp = pack_params(vs, vl);
+        uint8_t *rec = p.pages + record(slot / p.page_size, slot % p.page_size, ch / p.W, p.D / p.W,
+                                        p.page_size, p.W);
+        const int c = ch % p.W;
+        *reinterpret_cast<uint2 *>(rec + c) = make_uint2(kc, vc);
+        if (c % 32 == 0) *reinterpret_cast<uint2 *>(rec + p.W + c / 4) = make_uint2(kp, vp);
+        if (p.vk) {
+            values8(kc, kp, k);
+            values8(vc, vp, v);
+            store8(static_cast<T *>(p.vk) + row * p.ldv + ch, k);
+            store8(static_cast<T *>(p.vv) + row * p.ldv + ch, v);
+        }
+    }
+}
+
+struct Decode {
+    const void *qkv;  // [B, 3*D] rows: q | k | v
+    int64_t ldq;
+    const float *w;  // bias of head h: w + h * wh, row t at t * ldw
+    int64_t ldw, wh;
+    uint8_t *pages;
+    const int32_t *table;
+    int64_t ldtab;
+    const int32_t *pos;
+    int B, D, hs, W, nslab, n_pages, page_size, cap;
+    void *Z;
+    int64_t ldz;
+    int *status;
+};
+
+__device__ __forceinline__ float sigm(float q) { return 1.0f / (1.0f + __expf(-q)); }
+
+// Larger of two, NaN if either is: a NaN in the history reaches Z.
+__device__ __forceinline__ float fmax_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+constexpr int kWarps = 4;
+
+// One block per (sequence, slab).  A row's W channels are W/8 lanes, so a
+// warp reads 256/W rows at once; the warps' running (max, num, den) per
+// channel meet in shared memory.
+template <typename T, int LPR>
+__global__ void __launch_bounds__(32 * kWarps) decode_kernel(Decode p)
+{
+    grid_dep_wait();  // programmatic dependent launch: inputs are ready
+    grid_dep_launch();
+    constexpr int RPW = 32 / LPR;
+    const int b = blockIdx.x / p.nslab, slab = blockIdx.x % p.nslab;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = lane / LPR, oct = lane % LPR;
+    const int ch = slab * p.W + oct * 8;
+    T *z = static_cast<T *>(p.Z) + b * p.ldz + ch;
+    const int t = p.pos[b];
+    const float zero[8] = {};
+    if (t < 0 || t >= p.cap) {  // an inactive row
+        if (t >= 0 && threadIdx.x == 0) atomicOr(p.status, DC_DEVERR_FULL);
+        if (threadIdx.x < LPR) store8(z, zero);
+        return;
+    }
+    const int32_t *tab = p.table + b * p.ldtab;
+    const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + ch;
+    if (warp == 0) {  // append position t
+        float k[8], v[8], ks, kl, vs, vl;
+        load8(row + p.D, k);
+        load8(row + 2 * p.D, v);
+        const uint32_t kc = quantise8(k, ks, kl), vc = quantise8(v, vs, vl);
+        const int page = tab[t / p.page_size];
+        if (page < 0 || page >= p.n_pages) {
+            if (lane == 0) atomicOr(p.status, DC_DEVERR_PAGE);
+        } else if (sub == 0) {
+            uint8_t *rec = p.pages + record(page, t % p.page_size, slab, p.nslab, p.page_size, p.W);
+            *reinterpret_cast<uint2 *>(rec + oct * 8) = make_uint2(kc, vc);
+            if (oct % 4 == 0)
+                *reinterpret_cast<uint2 *>(rec + p.W + oct * 2) =
+                    make_uint2(pack_params(ks, kl), pack_params(vs, vl));
+        }
+    }
+    __syncthreads();
+    const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
+    float m[8], num[8], den[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        m[j] = -INFINITY;
+        num[j] = den[j] = 0.f;
+    }
+    for (int i = warp * RPW + sub; i <= t; i += kWarps * RPW) {
+        const int page = tab[i / p.page_size];
+        if (page < 0 || page >= p.n_pages) {
+            if (oct == 0) atomicOr(p.status, DC_DEVERR_PAGE);
+            continue;
+        }
+        const uint8_t *rec = p.pages + record(page, i % p.page_size, slab, p.nslab, p.page_size, p.W);
+        const uint2 code = *reinterpret_cast<const uint2 *>(rec + oct * 8);
+        const uint2 par = *reinterpret_cast<const uint2 *>(rec + p.W + oct / 4 * 8);
+        const float wi = w[i];
+        float k[8], v[8];
+        values8(code.x, par.x, k);
+        values8(code.y, par.y, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = k[j] + wi;
+            const float mx = fmax_nan(m[j], x);
+            if (mx == -INFINITY) continue;  // masked so far
+            const float scale = __expf(m[j] - mx), e = __expf(x - mx);
+            num[j] = num[j] * scale + e * v[j];
+            den[j] = den[j] * scale + e;
+            m[j] = mx;
+        }
+    }
+    // rows of a warp, then warps
+    auto join = [](float &m, float &num, float &den, float m2, float num2, float den2) {
+        const float mx = fmax_nan(m, m2);
+        if (mx == -INFINITY) return;
+        const float a = __expf(m - mx), c = __expf(m2 - mx);
+        num = num * a + num2 * c;
+        den = den * a + den2 * c;
+        m = mx;
+    };
+#pragma unroll
+    for (int o = LPR; o < 32; o *= 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            join(m[j], num[j], den[j], __shfl_xor_sync(0xffffffffu, m[j], o),
+                 __shfl_xor_sync(0xffffffffu, num[j], o), __shfl_xor_sync(0xffffffffu, den[j], o));
+    __shared__ float part[kWarps][3][8][LPR];
+    if (sub == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            part[warp][0][j][oct] = m[j];
+            part[warp][1][j][oct] = num[j];
+            part[warp][2][j][oct] = den[j];
+        }
+    __syncthreads();
+    if (threadIdx.x >= LPR) return;
+    for (int k = 1; k < kWarps; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            join(m[j], num[j], den[j], part[k][0][j][oct], part[k][1][j][oct], part[k][2][j][oct]);
+    float q[8];
+    load8(row, q);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = den[j] == 0.f ? 0.f : sigm(q[j]) * (num[j] / den[j]);
+    store8(z, q);
+}
+
+template <typename T>
+static cudaError_t launch_decode(const Decode &p, cudaStream_t st)
+{
+    const dim3 grid((unsigned)(p.B * p.nslab)), block(32 * kWarps);
+    switch (p.W) {
+        case 256: return launch_pdl(decode_kernel<T, 32>, grid, block, 0, st, 1, p);
+        case 128: return launch_pdl(decode_kernel<T, 16>, grid, block, 0, st, 1, p);
+        case 64: return launch_pdl(decode_kernel<T, 8>, grid, block, 0, st, 1, p);
+        default: return launch_pdl(decode_kernel<T, 4>, grid, block, 0, st, 1, p);
+    }
+}
+
+static int check_pool(int D, int n_pages, int page_size)
+{
+    if (D <= 0 || D % 32) return fail(DC_ERR_INVALID, "D must be a positive multiple of 32 (got %d)", D);
+    if (n_pages <= 0) return fail(DC_ERR_INVALID, "n_pages must be positive");
+    if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
+        return fail(DC_ERR_INVALID, "page_size must be 8, 16, 32, 64, 128 or 256 (got %d)", page_size);
+    if ((int64_t)n_pages * page_size > INT32_MAX)
+        return fail(DC_ERR_INVALID, "n_pages * page_size must be below 2^31");
+    return DC_OK;
+}
+
+}  // namespace kv4
+}  // namespace dc
+
+using namespace dc;
+
+extern "C" {
+
+int dc_kv4_pages_size(int n_pages, int page_size, int D, size_t *bytes)
+{
+    clear_error();
+    DC_TRY(kv4::check_pool(D, n_pages, page_size));
+    if (!bytes) return fail(DC_ERR_INVALID, "null pointer");
+    *bytes = (size_t)n_pages * page_size * D / 4 * 5;
+    return DC_OK;
+}
+
+int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t *slots, int n, int D,
+                 void *pages, int n_pages, int page_size, void *values_k, void *values_v, int ldv,
+                 void *stream)
+{
+    using namespace dc::kv4;
+    clear_error();
+    DC_TRY(check_pool(D, n_pages, page_size));
+    if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
+    if (n < 0) return fail(DC_ERR_INVALID, "bad row count %d", n);
+    if (n == 0) return DC_OK;
+    if (!k || !v || !slots || !pages) return fail(DC_ERR_INVALID, "null pointer");
+    if (!values_k != !values_v) return fail(DC_ERR_INVALID, "values_k and values_v go together");
+    const int per16 = dtype == DC_F32 ? 4 : 8;
+    if (ld < D || ld % per16 || (values_k && (ldv < D || ldv % per16)))
+        return fail(DC_ERR_INVALID, "row strides must be at least D and multiples of 16 bytes");
+    if (!aligned16(k) || !aligned16(v) || !aligned16(pages) || !aligned16(values_k) || !aligned16(values_v))
+        return fail(DC_ERR_INVALID, "k, v, pages and the values need 16-byte alignment");
+    Write p{};
+    p.k = k;
+    p.v = v;
+    p.ld = ld;
+    p.slots = slots;
+    p.n = n;
+    p.D = D;
+    p.W = slab_width(D);
+    p.page_size = page_size;
+    p.n_pages = n_pages;
+    p.pages = static_cast<uint8_t *>(pages);
+    p.vk = values_k;
+    p.vv = values_v;
+    p.ldv = ldv;
+    p.status = device_status_word();
+    if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
+    cudaStream_t st = as_stream(stream);
+    KernelTimer kt("kv4_write", st);
+    const int64_t blocks = ((int64_t)n * (D / 8) + 255) / 256;
+    const dim3 grid((unsigned)std::min<int64_t>(blocks, (int64_t)sm_count() * 64));
+    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(write_kernel<float>, grid, dim3(256), 0, st, 1, p)
+                                : launch_pdl(write_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, 1, p));
+    return DC_OK;
+}
+
+size_t dc_aft_decode4_workspace_size(int B, int D)
+{
+    if (B <= 0 || D <= 0) return 0;
+    return 256;
+}
+
+int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw, long long head_stride_w,
+                   void *pages, int n_pages, int page_size, const int32_t *table, int ldtab, int B, int H,
+                   int hs, const int32_t *pos, int Tmax, void *Z, int ldz, void *workspace,
+                   size_t workspace_bytes, void *stream)
+{
+    using namespace dc::kv4;
+    clear_error();
+    if (B < 0 || H <= 0 || hs <= 0 || Tmax <= 0 || ldtab <= 0 || (int64_t)H * hs > INT32_MAX / 4)
+        return fail(DC_ERR_INVALID, "bad decode shape B=%d H=%d hs=%d Tmax=%d ldtab=%d", B, H, hs, Tmax, ldtab);
+    const int D = H * hs;
+    DC_TRY(check_pool(D, n_pages, page_size));
+    if (hs % 8) return fail(DC_ERR_INVALID, "hs must be a multiple of 8 (got %d)", hs);
+    if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
+    if (B == 0) return DC_OK;
+    const int per16 = dtype == DC_F32 ? 4 : 8;
+    if (ldq < 3 * D || ldq % per16 || ldz < D || ldz % per16 || ldw < Tmax)
+        return fail(DC_ERR_INVALID, "ldq >= 3D and ldz >= D must be multiples of 16 bytes, ldw >= Tmax");
+    if (!qkv || !w || !pages || !table || !pos || !Z || !workspace) return fail(DC_ERR_INVALID, "null pointer");
+    if (!aligned16(qkv) || !aligned16(pages) || !aligned16(Z) || !aligned16(workspace))
+        return fail(DC_ERR_INVALID, "qkv, pages, Z and the workspace need 16-byte alignment");
+    if (workspace_bytes < dc_aft_decode4_workspace_size(B, D))
+        return fail(DC_ERR_NOMEM, "decode workspace too small");
+    Decode p{};
+    p.qkv = qkv;
+    p.ldq = ldq;
+    p.w = w;
+    p.ldw = ldw;
+    p.wh = head_stride_w;
+    p.pages = static_cast<uint8_t *>(pages);
+    p.table = table;
+    p.ldtab = ldtab;
+    p.pos = pos;
+    p.B = B;
+    p.D = D;
+    p.hs = hs;
+    p.W = slab_width(D);
+    p.nslab = D / p.W;
+    p.n_pages = n_pages;
+    p.page_size = page_size;
+    p.cap = (int)std::min<int64_t>(Tmax, (int64_t)ldtab * page_size);
+    p.Z = Z;
+    p.ldz = ldz;
+    p.status = device_status_word();
+    if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
+    if ((int64_t)B * p.nslab > INT32_MAX) return fail(DC_ERR_INVALID, "B * D too large");
+    cudaStream_t st = as_stream(stream);
+    KernelTimer kt("aft_decode4", st);
+    DC_CUDA_TRY(dtype == DC_F32 ? launch_decode<float>(p, st) : launch_decode<__nv_bfloat16>(p, st));
+    return DC_OK;
+}
+
+}  // extern "C"

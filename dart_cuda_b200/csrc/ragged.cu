@@ -1,0 +1,462 @@
+// Kernels of a generation batch whose sequences have lengths of their own:
+//
+//   page_tables       block tables and slot maps from request lengths
+//   logits_controls   penalties for repeated tokens, biases, grammar masks
+//   greedy_embed_rows argmax and next embedding, a position per row
+//
+// The reference samples on the host, one sequence at a time, after copying
+// the logits back (example/bin/shakespear4.dart:176-216) and has none of
+// these.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "dc_internal.h"
+#include "dc_ptx.cuh"
+
+namespace dc {
+namespace ragged {
+
+constexpr int DC_DEVERR_INDEX = 0x20;   // a token id outside [0, V)
+constexpr int DC_DEVERR_FULL = 0x40;    // decode ran past the sequence capacity
+constexpr int DC_DEVERR_POOL = 0x100;   // no page for a token: free list or table row used up
+
+// ------------------------------------------------------------ page tables
+// Request b has start tokens in pages listed in its table row and gets count
+// more: have = ceil(start / ps) pages are there, last = ceil((start + count) /
+// ps) (at most the row's length) are needed, and the missing ones are taken
+// from the free list in request order, at head + the sum of what earlier
+// requests take.  Every page is thus known by arithmetic from two prefix
+// sums, so table entries and slots are written independently of each other.
+constexpr int kTabThreads = 1024;
+
+struct Tables {
+    const int32_t *start, *count;
+    int B, shift;
+    const int32_t *free_pages;
+    int n_free;
+    const int32_t *head;
+    int32_t *head_out, *table;
+    int ldtab;
+    int32_t *slots;
+    int n_slots, ld_slots;
+    int32_t *row_start;
+    int *status;
+};
+
+// Exclusive prefix sums of two values over the block, and their totals.
+__device__ __forceinline__ void scan2(int64_t &a, int &b, int64_t &ta, int &tb)
+{
+    __shared__ int64_t wa[32];
+    __shared__ int wb[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t ia = a;
+    int ib = b;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t ua = __shfl_up_sync(0xffffffffu, ia, o);
+        const int ub = __shfl_up_sync(0xffffffffu, ib, o);
+        if (lane >= o) {
+            ia += ua;
+            ib += ub;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) {
+        wa[warp] = ia;
+        wb[warp] = ib;
+    }
+    __syncthreads();
+    int64_t sa = lane < (int)(blockDim.x >> 5) ? wa[lane] : 0;
+    int sb = lane < (int)(blockDim.x >> 5) ? wb[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t ua = __shfl_up_sync(0xffffffffu, sa, o);
+        const int ub = __shfl_up_sync(0xffffffffu, sb, o);
+        if (lane >= o) {
+            sa += ua;
+            sb += ub;
+        }
+    }
+    ta = __shfl_sync(0xffffffffu, sa, 31);
+    tb = __shfl_sync(0xffffffffu, sb, 31);
+    const int64_t before_a = __shfl_sync(0xffffffffu, sa, (warp + 31) & 31);
+    const int before_b = __shfl_sync(0xffffffffu, sb, (warp + 31) & 31);
+    a = ia - a + (warp ? before_a : 0);
+    b = ib - b + (warp ? before_b : 0);
+}
+
+__global__ void __launch_bounds__(kTabThreads) tables_kernel(Tables p)
+{
+    grid_dep_wait();  // programmatic dependent launch: inputs are ready
+    grid_dep_launch();
+    // requests of this round: first token, tokens, pages there and needed,
+    // free page of table column 0 (column c >= have takes free[base + c]),
+    // packed row
+    __shared__ int s_start[kTabThreads], s_count[kTabThreads], s_have[kTabThreads], s_last[kTabThreads],
+        s_base[kTabThreads];
+    __shared__ int64_t s_row[kTabThreads + 1];
+    const int ps = 1 << p.shift, tid = threadIdx.x;
+    const int head = min(max(0, *p.head), p.n_free);
+    int64_t rows = 0;
+    int pages = 0, err = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kTabThreads) {
+        const int b = b0 + tid, nb = min(kTabThreads, p.B - b0);
+        int start = 0, count = 0, have = 0, last = 0;
+        if (b < p.B) {
+            start = p.start[b];
+            count = start < 0 ? 0 : max(0, p.count[b]);
+            start = max(0, start);
+            have = (int)(((int64_t)start + ps - 1) >> p.shift);
+            const int64_t want = ((int64_t)start + count + ps - 1) >> p.shift;
+            if (count && want > p.ldtab) err = 1;
+            last = (int)min((int64_t)p.ldtab, want);
+        }
+        const int need = max(0, last - have);
+        int64_t row = count, trow;
+        int first = need, tpages;
+        scan2(row, first, trow, tpages);
+        s_start[tid] = start;
+        s_count[tid] = count;
+        s_have[tid] = have;
+        s_last[tid] = last;
+        s_row[tid] = rows + row;
+        s_base[tid] = (int)min((int64_t)INT32_MAX / 2, (int64_t)head + pages + first) - have;
+        if (tid == 0) s_row[nb] = rows + trow;
+        if (b < p.B && p.row_start) p.row_start[b] = (int)min(rows + row, (int64_t)INT32_MAX);
+        if (need && (int64_t)head + pages + first + need > p.n_free) err = 1;
+        __syncthreads();
+        // table entries: a warp per request
+        for (int r = tid >> 5; r < nb; r += kTabThreads / 32) {
+            for (int c = s_have[r] + (tid & 31); c < s_last[r]; c += 32) {
+                const int at = s_base[r] + c;
+                p.table[(int64_t)(b0 + r) * p.ldtab + c] = at < p.n_free ? p.free_pages[at] : -1;
+            }
+        }
+        // slots: token j of request r
+        auto slot_of = [&](int r, int j) {
+            const int64_t t = (int64_t)s_start[r] + j;
+            const int64_t c = t >> p.shift;
+            if (c >= p.ldtab) return -1;
+            const int at = s_base[r] + (int)c;
+            int page = -1;
+            if (c < s_have[r])  // the page that start ends in
+                page = p.table[(int64_t)(b0 + r) * p.ldtab + c];
+            else if (at < p.n_free)
+                page = p.free_pages[at];
+            const int64_t slot = (int64_t)page * ps + (t & (ps - 1));
+            if (page < 0 || slot > INT32_MAX) {
+                err = 1;
+                return -1;
+            }
+            return (int)slot;
+        };
+        if (p.slots && p.ld_slots) {
+            const int64_t i0 = (int64_t)b0 * p.ld_slots, i1 = (int64_t)(b0 + nb) * p.ld_slots;
+            for (int64_t i = i0 + tid; i < i1; i += kTabThreads) {
+                const int r = (int)((i - i0) / p.ld_slots), j = (int)((i - i0) % p.ld_slots);
+                p.slots[i] = j < s_count[r] ? slot_of(r, j) : -1;
+            }
+            if (b < p.B && count > p.ld_slots) err = 1;
+        } else if (p.slots) {
+            for (int64_t i = s_row[0] + tid; i < min(s_row[nb], (int64_t)p.n_slots); i += kTabThreads) {
+                int lo = 0, hi = nb - 1;  // last request that starts at or before i
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (s_row[mid] <= i) lo = mid;
+                    else hi = mid - 1;
+                }
+                p.slots[i] = slot_of(lo, (int)(i - s_row[lo]));
+            }
+            if (s_row[nb] > p.n_slots) err = 1;
+        }
+        rows += trow;
+        pages += tpages;
+        __syncthreads();
+    }
+    if (p.slots) {  // behind the last token
+        const int64_t used = p.ld_slots ? (int64_t)p.B * p.ld_slots : rows;
+        for (int64_t i = used + tid; i < p.n_slots; i += kTabThreads) p.slots[i] = -1;
+    }
+    if (tid == 0) {
+        if (p.row_start) p.row_start[p.B] = (int)min(rows, (int64_t)INT32_MAX);
+        *p.head_out = (int)min((int64_t)p.n_free, (int64_t)head + pages);
+    }
+    if (err) atomicOr(p.status, DC_DEVERR_POOL);
+}
+
+// ------------------------------------------------------------ logits
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+struct Logits {
+    const void *in;
+    void *out;
+    int64_t ldl, ldo;
+    int B, V, chunk, chunks;
+    const int32_t *tokens;
+    int ldt;
+    const int32_t *pos;
+    int pos_stride;
+    const int32_t *prompt;
+    const float *rep, *pres, *freq, *bias;
+    int64_t ldb;
+    const uint32_t *mask;
+    int64_t ldm;
+};
+
+constexpr uint32_t kSeen = 0x80000000u;
+
+// One block per chunk of a row's vocabulary: the tokens known so far that
+// fall into the chunk are counted in shared memory (bit 31: seen in the
+// prompt; the rest: how often generated), then the logits stream through.
+template <typename T>
+__global__ void __launch_bounds__(256) logits_kernel(Logits p)
+{
+    grid_dep_wait();  // programmatic dependent launch: inputs are ready
+    grid_dep_launch();
+    extern __shared__ uint32_t hist[];
+    const int b = blockIdx.x / p.chunks, v0 = blockIdx.x % p.chunks * p.chunk;
+    const int n = min(p.chunk, p.V - v0);
+    const bool pens = p.rep || p.pres || p.freq;
+    if (pens) {
+        for (int i = threadIdx.x; i < n; i += blockDim.x) hist[i] = 0;
+        __syncthreads();
+        const int known = min(p.ldt, p.pos[(int64_t)b * p.pos_stride] + 1);
+        const int prompt = p.prompt ? p.prompt[b] : 0;
+        const int32_t *tok = p.tokens + (int64_t)b * p.ldt;
+        for (int i = threadIdx.x; i < known; i += blockDim.x) {
+            const uint32_t v = (uint32_t)(tok[i] - v0);
+            if (v < (uint32_t)n) {
+                if (i < prompt) atomicOr(hist + v, kSeen);
+                else atomicAdd(hist + v, 1u);
+            }
+        }
+        __syncthreads();
+    }
+    const float rep = p.rep ? p.rep[b] : 1.f, pres = p.pres ? p.pres[b] : 0.f, freq = p.freq ? p.freq[b] : 0.f;
+    const T *in = static_cast<const T *>(p.in) + b * p.ldl + v0;
+    T *out = static_cast<T *>(p.out) + b * p.ldo + v0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        float x = to_f<T>(in[i]);
+        const uint32_t h = pens ? hist[i] : 0;
+        if (h) {
+            if (p.rep) x = x > 0.f ? x / rep : x * rep;
+            const uint32_t made = h & ~kSeen;
+            if (made) x = (x - freq * (float)made) - pres;
+        }
+        if (p.bias) x += p.bias[b * p.ldb + v0 + i];
+        if (p.mask && !(p.mask[b * p.ldm + (v0 + i) / 32] >> ((v0 + i) & 31) & 1u)) x = -INFINITY;
+        out[i] = from_f<T>(x);
+    }
+}
+
+// ------------------------------------------------------------ pick
+struct Pick {
+    const void *logits;
+    int64_t ldl;
+    int B, V;
+    const float *wte, *wpe;
+    const int32_t *pos;
+    int32_t *pos_out;
+    int D;
+    int32_t *tokens;
+    int ldt;
+    float *x;
+    int *status;
+};
+
+// One block per row: argmax (lowest index on ties, NaN never wins), the
+// token's embedding at the row's next position, the advanced position.
+template <typename T>
+__global__ void __launch_bounds__(256) pick_kernel(Pick p)
+{
+    grid_dep_wait();  // programmatic dependent launch: inputs are ready
+    grid_dep_launch();
+    __shared__ float sv[8];
+    __shared__ int si[8];
+    const int b = blockIdx.x;
+    const int at = p.pos[b];
+    __syncthreads();  // pos_out may be pos: every thread has read its position
+    if (at < 0 || at >= p.ldt - 1) {
+        if (threadIdx.x == 0) {
+            p.pos_out[b] = at;
+            if (at >= 0) atomicOr(p.status, DC_DEVERR_FULL);
+        }
+        return;
+    }
+    const T *l = static_cast<const T *>(p.logits) + b * p.ldl;
+    float best = -INFINITY;
+    int bi = 0x7fffffff;
+    auto take = [&](float x, int v) {
+        if (x > best || (x == best && v < bi)) {
+            best = x;
+            bi = v;
+        }
+    };
+    for (int v = threadIdx.x; v < p.V; v += blockDim.x) take(to_f<T>(l[v]), v);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float ov = __shfl_xor_sync(0xffffffffu, best, o);
+        const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+        take(ov, oi);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sv[threadIdx.x >> 5] = best;
+        si[threadIdx.x >> 5] = bi;
+    }
+    __syncthreads();
+    for (int k = 0; k < 8; ++k) take(sv[k], si[k]);
+    const int tok = bi < p.V ? bi : 0;  // all NaN: token 0
+    if (threadIdx.x == 0) {
+        p.tokens[(int64_t)b * p.ldt + at + 1] = tok;
+        p.pos_out[b] = at + 1;
+    }
+    if (p.x) {
+        const float *e = p.wte + (int64_t)tok * p.D, *q = p.wpe + (int64_t)(at + 1) * p.D;
+        for (int d = threadIdx.x; d < p.D; d += blockDim.x) p.x[(int64_t)b * p.D + d] = e[d] + q[d];
+    }
+}
+
+}  // namespace ragged
+}  // namespace dc
+
+using namespace dc;
+using namespace dc::ragged;
+
+extern "C" {
+
+int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_size, const int32_t *free_pages,
+                   int n_free, const int32_t *free_head, int32_t *free_head_out, int32_t *table, int ldtab,
+                   int32_t *slots, int n_slots, int ld_slots, int32_t *row_start, void *stream)
+{
+    clear_error();
+    if (B < 0 || n_free < 0 || ldtab <= 0 || n_slots < 0 || ld_slots < 0)
+        return fail(DC_ERR_INVALID, "bad shape B=%d n_free=%d ldtab=%d n_slots=%d ld_slots=%d", B, n_free, ldtab,
+                    n_slots, ld_slots);
+    if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
+        return fail(DC_ERR_INVALID, "page_size must be 8, 16, 32, 64, 128 or 256 (got %d)", page_size);
+    if ((int64_t)B * ldtab > INT32_MAX) return fail(DC_ERR_INVALID, "B * ldtab must be below 2^31");
+    if (B == 0) return DC_OK;
+    if (!start || !count || !free_pages || !free_head || !free_head_out || !table)
+        return fail(DC_ERR_INVALID, "null pointer");
+    if (slots && ld_slots && (int64_t)B * ld_slots > n_slots)
+        return fail(DC_ERR_INVALID, "slots holds %d, B * ld_slots is %lld", n_slots, (long long)B * ld_slots);
+    Tables p{};
+    p.start = start;
+    p.count = count;
+    p.B = B;
+    for (p.shift = 3; 1 << p.shift < page_size;) ++p.shift;
+    p.free_pages = free_pages;
+    p.n_free = n_free;
+    p.head = free_head;
+    p.head_out = free_head_out;
+    p.table = table;
+    p.ldtab = ldtab;
+    p.slots = slots;
+    p.n_slots = n_slots;
+    p.ld_slots = ld_slots;
+    p.row_start = row_start;
+    p.status = device_status_word();
+    if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
+    cudaStream_t st = as_stream(stream);
+    KernelTimer kt("page_tables", st);
+    DC_CUDA_TRY(launch_pdl(tables_kernel, dim3(1), dim3(kTabThreads), 0, st, 1, p));
+    return DC_OK;
+}
+
+int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtype, int B, int V,
+                       const int32_t *tokens, int ldt, const int32_t *pos, int pos_stride,
+                       const int32_t *prompt_len, const float *repetition, const float *presence,
+                       const float *frequency, const float *bias, int ldb, const uint32_t *mask, int ldm,
+                       void *stream)
+{
+    clear_error();
+    if (B < 0 || V <= 0 || ldl < V || ldo < V) return fail(DC_ERR_INVALID, "bad shape B=%d V=%d", B, V);
+    if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
+    if (B == 0) return DC_OK;
+    if (!logits || !out) return fail(DC_ERR_INVALID, "null pointer");
+    if (logits == out && ldl != ldo) return fail(DC_ERR_INVALID, "in place needs one row stride");
+    const bool pens = repetition || presence || frequency;
+    if (pens && (!tokens || !pos || ldt <= 0 || (pos_stride != 0 && pos_stride != 1)))
+        return fail(DC_ERR_INVALID, "penalties need the tokens and positions (pos_stride 0 or 1)");
+    if (bias && ldb != 0 && ldb < V) return fail(DC_ERR_INVALID, "ldb must be 0 (one bias) or at least V");
+    if (mask && ldm != 0 && ldm < (V + 31) / 32)
+        return fail(DC_ERR_INVALID, "ldm must be 0 (one mask) or at least ceil(V / 32)");
+    Logits p{};
+    p.in = logits;
+    p.out = out;
+    p.ldl = ldl;
+    p.ldo = ldo;
+    p.B = B;
+    p.V = V;
+    p.chunk = 4096;
+    p.chunks = (V + p.chunk - 1) / p.chunk;
+    p.tokens = tokens;
+    p.ldt = ldt;
+    p.pos = pos;
+    p.pos_stride = pos_stride;
+    p.prompt = prompt_len;
+    p.rep = repetition;
+    p.pres = presence;
+    p.freq = frequency;
+    p.bias = bias;
+    p.ldb = ldb;
+    p.mask = mask;
+    p.ldm = ldm;
+    if ((int64_t)B * p.chunks > INT32_MAX) return fail(DC_ERR_INVALID, "B * V too large");
+    cudaStream_t st = as_stream(stream);
+    KernelTimer kt("logits_controls", st);
+    const dim3 grid((unsigned)(B * p.chunks));
+    const size_t smem = pens ? p.chunk * sizeof(uint32_t) : 0;
+    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(logits_kernel<float>, grid, dim3(256), smem, st, 1, p)
+                                : launch_pdl(logits_kernel<__nv_bfloat16>, grid, dim3(256), smem, st, 1, p));
+    return DC_OK;
+}
+
+int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, const float *wte,
+                         const float *wpe, const int32_t *pos, int32_t *pos_out, int D, int32_t *tokens,
+                         int ldt, float *x, void *stream)
+{
+    clear_error();
+    if (B < 0 || V <= 0 || ldl < V || ldt <= 0) return fail(DC_ERR_INVALID, "bad shape B=%d V=%d ldt=%d", B, V, ldt);
+    if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
+    if (B == 0) return DC_OK;
+    if (!logits || !pos || !pos_out || !tokens) return fail(DC_ERR_INVALID, "null pointer");
+    if (x && (!wte || !wpe || D <= 0)) return fail(DC_ERR_INVALID, "embedding tables needed");
+    Pick p{};
+    p.logits = logits;
+    p.ldl = ldl;
+    p.B = B;
+    p.V = V;
+    p.wte = wte;
+    p.wpe = wpe;
+    p.pos = pos;
+    p.pos_out = pos_out;
+    p.D = D;
+    p.tokens = tokens;
+    p.ldt = ldt;
+    p.x = x;
+    p.status = device_status_word();
+    if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
+    cudaStream_t st = as_stream(stream);
+    KernelTimer kt("greedy_embed_rows", st);
+    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(pick_kernel<float>, dim3(B), dim3(256), 0, st, 1, p)
+                                : launch_pdl(pick_kernel<__nv_bfloat16>, dim3(B), dim3(256), 0, st, 1, p));
+    return DC_OK;
+}
+
+}  // extern "C"

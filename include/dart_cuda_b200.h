@@ -93,7 +93,11 @@ const char *dc_last_error(void);
  *              is below 2^-100 (e.g. a row's w and a column's K rising in
  *              opposite directions over a combined spread of about 70 or
  *              more), that output and its gradients are not reliable and this
- *              bit is set instead of the error passing silently. */
+ *              bit is set instead of the error passing silently.
+ *   0x100      dc_page_tables had no page for a token (the free list or a
+ *              table row is used up); the token's slot is -1
+ *   0x200      a slot or a page id outside the pool of a paged history; the
+ *              row was not written, or the page's positions were left out */
 #define DC_STATUS_AFT_RANGE 0x80
 int dc_device_status(void *stream, int *bits);
 
@@ -315,6 +319,96 @@ int dc_aft_decode(const float *qkv, int ldq, const float *w, int ldw, long long 
                   void *workspace, size_t workspace_bytes, void *stream);
 /* Fill cache rows [0, T) from a prefill's fused projection [B*T, 3D]. */
 int dc_kv_cache_fill(const float *qkv, int ldq, int B, int T, int D, float *cache, void *stream);
+
+/* -------------------------------------------------- ragged generation
+ * A generation batch whose sequences have lengths of their own, over a paged
+ * k/v history held in 4 bits.  None of these has a counterpart in the
+ * reference, which generates one sequence at a time from the whole context
+ * (example/bin/shakespear4.dart:176-216).
+ *
+ * Block tables and slot maps from request lengths.  Request b holds start[b]
+ * tokens in the pages that row b of table [B, ldtab] lists and gets count[b]
+ * more (start < 0 or count <= 0: none).  The pages it lacks are taken from
+ * free_pages[n_free] in request order, from *free_head on, and entered in
+ * its row (other entries stay); *free_head_out, which may be free_head,
+ * receives the next unused one.  Token j of request b is the slot
+ * page * page_size + offset of position start[b] + j, written to
+ * slots[row_start[b] + j] (packed, ld_slots = 0) or slots[b * ld_slots + j];
+ * entries of slots [n_slots] that belong to no token become -1.  row_start
+ * [B + 1] receives the prefix sums of the counts.  slots and row_start may be
+ * NULL.  A token for which there is no page left gets -1 and sets status bit
+ * 0x100.  page_size: 8, 16, 32, 64, 128 or 256. */
+int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_size,
+                   const int32_t *free_pages, int n_free, const int32_t *free_head,
+                   int32_t *free_head_out, int32_t *table, int ldtab, int32_t *slots, int n_slots,
+                   int ld_slots, int32_t *row_start, void *stream);
+
+/* Paged 4-bit history of one layer: n_pages pages of page_size positions of D
+ * channels (a multiple of 32), dc_kv4_pages_size bytes, 16-byte aligned:
+ * [n_pages][D/W][page_size][5W/4], W the largest of 256, 128, 64, 32 that
+ * divides D.  A record holds, per 8 channels, 4 bytes of k codes and 4 of v
+ * codes (channel j in bits 4j..4j+3), then per group of 32 channels four
+ * bf16: k step, k low, v step, v low.  Code c stands for low + step * c, with
+ * low the largest bf16 <= the group's minimum, step the smallest bf16 >=
+ * (maximum - low) / 15 and c = floor((x - low) / step + 1/2), so a value is
+ * off by at most step / 2.  A group with a value that is not finite, or
+ * above 1e38 in magnitude, reads as NaN.
+ *
+ * dc_kv4_write quantises n rows of k and v (row stride ld, `dtype`, 16-byte
+ * aligned rows) into the slots slots[n]; rows whose slot is negative are left
+ * out.  Slots of one call must differ from each other.  values_k, values_v
+ * (row stride ldv, may be k and v themselves, NULL: not wanted) receive what
+ * the stored codes stand for, in `dtype`. */
+int dc_kv4_pages_size(int n_pages, int page_size, int D, size_t *bytes);
+int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t *slots, int n,
+                 int D, void *pages, int n_pages, int page_size, void *values_k, void *values_v,
+                 int ldv, void *stream);
+
+/* dc_aft_decode over a paged 4-bit history, with a position t = pos[b] of its
+ * own for every sequence: qkv [B, 3D] (q | k | v, row stride ldq, D = H * hs,
+ * hs a multiple of 8) in `dtype` is quantised and appended at position t
+ * through row b of table [B, ldtab], and Z[b,:] (row stride ldz, `dtype`)
+ * receives the AFT row over the positions 0..t that the history then holds.
+ * w is head h's bias at w + h * head_stride_w, row stride ldw >= Tmax.  A
+ * sequence with pos < 0 is left out and its Z row is zero; so is one with
+ * pos >= min(Tmax, ldtab * page_size), which sets status bit 0x40, and one
+ * whose bias row is -inf throughout.  Sequences may share pages they only
+ * read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
+ * zero-filled once before its first use (the kernel leaves it zeroed); calls
+ * that may overlap on the GPU need one each. */
+size_t dc_aft_decode4_workspace_size(int B, int D);
+int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
+                   long long head_stride_w, void *pages, int n_pages, int page_size,
+                   const int32_t *table, int ldtab, int B, int H, int hs, const int32_t *pos,
+                   int Tmax, void *Z, int ldz, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
+/* Logits of B rows before the pick: out[b,v] (row stride ldo; may be logits
+ * with ldo = ldl) = logits[b,v] (row stride ldl, `dtype`), where
+ *   v occurs in tokens[b, 0..p]:  x = x > 0 ? x / r : x * r
+ *   v occurs n > 0 times in tokens[b, prompt_len[b]..p]:  x -= f * n + q
+ *   bias:  x += bias[b * ldb + v]   (ldb = 0: one for all rows)
+ *   mask:  x = -inf where bit v % 32 of mask[b * ldm + v / 32] is 0
+ *                                   (ldm = 0: one for all rows)
+ * with p = pos[b * pos_stride] the position the logits belong to (pos_stride
+ * 0: one for all rows; p < 0: no tokens yet), tokens [B, ldt], and per row
+ * r = repetition[b] > 0, q = presence[b], f = frequency[b].  prompt_len NULL
+ * stands for 0; each other array may be NULL (without effect).  Token ids
+ * outside [0, V) are ignored.  A row whose mask allows nothing is all -inf. */
+int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtype, int B, int V,
+                       const int32_t *tokens, int ldt, const int32_t *pos, int pos_stride,
+                       const int32_t *prompt_len, const float *repetition, const float *presence,
+                       const float *frequency, const float *bias, int ldb, const uint32_t *mask,
+                       int ldm, void *stream);
+
+/* dc_greedy_embed with a position p = pos[b] of its own for every row and
+ * logits in `dtype`: tokens[b, p+1] = argmax (lowest index on ties), x[b,:] =
+ * wte[token,:] + wpe[p+1,:] when x is non-NULL (wpe: at least ldt rows), and
+ * pos_out[b] (may be pos) = p+1.  A row with p < 0 is left as it is; one with
+ * p+1 >= ldt too, and sets status bit 0x40. */
+int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, const float *wte,
+                         const float *wpe, const int32_t *pos, int32_t *pos_out, int D,
+                         int32_t *tokens, int ldt, float *x, void *stream);
 
 /* ------------------------------------------------------------------ legacy
  * The reference's handle ABI (native/src/engine.cu).  Every returned handle
