@@ -20,6 +20,9 @@ lib/core/layers/nn.dart) for B sequences per call instead of one:
   k/v history), then one cached decode step per new token, greedy.  The
   reference re-runs the whole context per token
   (example/bin/shakespear4.dart:176-214).
+  ``cache_bits=4`` keeps the history quantised in pages of a pool, for
+  prompts of different lengths (``lens``); ``controls`` are penalties for
+  repeated tokens, biases and a grammar mask applied before each pick.
 * ``save`` / ``load``: the reference's checkpoint, flat fp32 in its
   ``parameters()`` order (lib/core/utils/persistence.dart:8-70).
 
@@ -74,6 +77,35 @@ class DecoderConfig:
     @property
     def enc(self):
         return self.enc_dim or self.d_model
+
+
+@dataclass
+class LogitControls:
+    """What ``generate`` does to the logits before each pick
+    (``ops.logits_controls``).  repetition, presence, frequency: a number, or
+    one per sequence; bias: [V] or [B, V] fp32; mask: packed int32 words
+    [ceil(V/32)] or [B, ceil(V/32)], bit set = token allowed.  The presence and
+    frequency penalties count generated tokens, the repetition penalty the
+    prompt's too.  A mask or bias on the device may be rewritten between
+    steps."""
+    repetition: object = None
+    presence: object = None
+    frequency: object = None
+    bias: torch.Tensor | None = None
+    mask: torch.Tensor | None = None
+
+    def on(self, B, device):
+        """Keyword arguments of ops.logits_controls for B sequences."""
+        def rows(x):
+            if x is None:
+                return None
+            return torch.as_tensor(x, dtype=torch.float32, device=device).expand(B).contiguous()
+
+        def put(x):
+            return None if x is None else x.to(device)
+
+        return dict(repetition=rows(self.repetition), presence=rows(self.presence), frequency=rows(self.frequency),
+                    bias=put(self.bias), mask=put(self.mask))
 
 
 class AftDecoder:
@@ -298,10 +330,12 @@ class AftDecoder:
         return self.P[f"{l}.bcv"]
 
     # ------------------------------------------------------------ training
-    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None, lm_head: bool = True):
+    def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None, lm_head: bool = True, on_qkv=None):
         """Logits [B*T, V] of token ids idx [B, T] (int32, on the device) and,
         with targets, the mean label-smoothed cross-entropy (device scalar).
-        Without ``lm_head`` the forward stops after the final LayerNorm."""
+        Without ``lm_head`` the forward stops after the final LayerNorm.
+        ``on_qkv(l, qkv)``, when given, is called between layer l's fused
+        projection [B*T, 3d] and its attention (a prefill stores k and v)."""
         c, P = self.cfg, self.P
         B, T = idx.shape
         b = self._buffers(B, T)
@@ -313,6 +347,8 @@ class AftDecoder:
             x = b["x"][l]
             ops.layernorm_fwd(x, P[f"{l}.ln1g"], P[f"{l}.ln1b"], out=b["a1"][l])
             ops.gemm(b["a1"][l], P[f"{l}.wqkv"], out=b["qkv"][l], bias=P[f"{l}.bqkv"])
+            if on_qkv is not None:
+                on_qkv(l, b["qkv"][l])
             self._aft(l, b["qkv"][l], b["z"][l], B, T)
             ops.gemm(b["z"][l], P[f"{l}.wo"], out=b["x1"][l], bias=P[f"{l}.bo"], residual=x)
             ops.layernorm_fwd(b["x1"][l], P[f"{l}.ln2g"], P[f"{l}.ln2b"], out=b["a2"][l])
@@ -484,67 +520,145 @@ class AftDecoder:
         return loss
 
     # ------------------------------------------------------------ decoding
-    def _decode_state(self, B):
-        if self._dec is not None and self._dec["B"] == B:
-            return self._dec
+    def _decode_state(self, B, bits=32, n_pages=0, page_size=16):
+        key = (B, bits, page_size if bits == 4 else 0)
+        s = self._dec
+        if s is not None and s["key"] == key and n_pages <= s.get("n_pages", 0):
+            return s
         c, dev = self.cfg, self.device
         d, F, Tm = c.d_model, c.ffn_mult * c.d_model, c.block_size
         z = lambda *s: torch.zeros(*s, device=dev)
-        s = {"B": B}
-        s["cache"] = [z(Tm, B * d * 2) for _ in range(c.n_layers)]
+        zi = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
+        s = {"B": B, "key": key, "controls": None}
         s["x"], s["a"], s["zd"], s["cg"] = (z(B, d) for _ in range(4))
         s["qkv"], s["h"] = z(B, 3 * d), z(B, F)
         s["logits"] = z(B, c.vocab)
         s["v0"] = [self.P[f"{l}.bcv"] for l in range(c.n_layers)]
-        s["tokens"] = torch.zeros(B, Tm, dtype=torch.int32, device=dev)
-        s["pos"] = torch.zeros(1, dtype=torch.int32, device=dev)
-        nb = lib().dc_aft_decode_workspace_size(B, d, Tm)
-        s["ws"] = torch.zeros(nb, dtype=torch.uint8, device=dev)  # counters start at zero
-        s["ws_bytes"] = nb
+        s["tokens"] = zi(B, Tm)
+        s["prompt_len"] = zi(B)
+        if bits == 4:
+            if d % 32 or c.head % 8:
+                raise ValueError("a 4-bit history needs d_model a multiple of 32 and heads of a multiple of 8 channels")
+            s["n_pages"], s["page_size"] = n_pages, page_size
+            s["cache"] = [ops.kv4_pages(n_pages, page_size, d, device=dev) for _ in range(c.n_layers)]
+            s["free"] = torch.arange(n_pages, dtype=torch.int32, device=dev)
+            s["head"], s["pos"], s["one"] = zi(1), zi(B), zi(B) + 1
+            s["table"] = zi(B, -(-Tm // page_size)) - 1
+            s["ws"] = ops.aft_decode4_workspace(B, d, device=dev)
+            s["w"] = [self.P[f"{l}.pos"] for l in range(c.n_layers)]
+        else:
+            s["cache"] = [z(Tm, B * d * 2) for _ in range(c.n_layers)]
+            s["pos"] = zi(1)
+            nb = lib().dc_aft_decode_workspace_size(B, d, Tm)
+            s["ws"] = torch.zeros(nb, dtype=torch.uint8, device=dev)  # counters start at zero
+            s["ws_bytes"] = nb
         self._dec = s
         return s
 
-    def prefill(self, prompt: torch.Tensor):
+    def prefill(self, prompt: torch.Tensor, lens=None, cache_bits=32, n_new=None, page_size=16,
+                controls: LogitControls | None = None):
         """Run the prompt [B, T0] (int32) through the batched forward, keep
-        every layer's k/v history and pick the first new token (greedy)."""
+        every layer's k/v history and pick the first new token (greedy).
+
+        cache_bits=4 keeps the history in 4 bits, in pages of page_size
+        positions taken from a pool that holds the prompts and n_new tokens a
+        sequence (by default, as many as fit the block size); the forward
+        attends to the k and v that the history stands for, as the steps
+        after it do.  lens (4 bits only): the prompts' lengths, 1..T0; what
+        follows a shorter prompt in its row must be valid token ids and is
+        otherwise ignored."""
         c, P = self.cfg, self.P
         B, T0 = prompt.shape
-        s = self._decode_state(B)
         d, V, Tm = c.d_model, c.vocab, c.block_size
+        if cache_bits not in (4, 32):
+            raise ValueError(f"cache_bits must be 4 or 32 (got {cache_bits})")
+        if lens is not None and cache_bits != 4:
+            raise ValueError("prompts of different lengths need cache_bits=4: the 32-bit history has one position")
+        if cache_bits == 4:
+            lens = [T0] * B if lens is None else [int(n) for n in lens]
+            if len(lens) != B or min(lens) < 1 or max(lens) > T0:
+                raise ValueError(f"lens must hold a length of 1..{T0} for each of the {B} prompts")
+            ends = [min(Tm, n + (Tm if n_new is None else n_new)) for n in lens]
+            s = self._decode_state(B, 4, sum(-(-n // page_size) for n in ends), page_size)
+            s["prompt_len"].copy_(torch.tensor(lens, dtype=torch.int32))
+        else:
+            s = self._decode_state(B)
+            s["prompt_len"].fill_(T0)
+        s["controls"] = None if controls is None else controls.on(B, self.device)
         st = ops._stream()
-        self.forward(prompt, lm_head=False)
-        b = self._bufs
-        for l in range(c.n_layers):
-            check(lib().dc_kv_cache_fill(b["qkv"][l].data_ptr(), 3 * d, B, T0, d, s["cache"][l].data_ptr(), st),
-                  "dc_kv_cache_fill")
-        # LM head on the last position only: rows b*T0 + T0-1 of the final LN
-        last = b["af"].view(B, T0, d)[:, T0 - 1, :]
+        if cache_bits == 4:
+            s["head"].zero_()
+            s["table"].fill_(-1)
+            s["pos"].zero_()  # no tokens yet
+            slots = torch.empty(B * T0, dtype=torch.int32, device=self.device)
+            ops.page_tables(s["pos"], s["prompt_len"], s["free"], s["head"], s["table"], page_size, slots=slots,
+                            ld_slots=T0)
+
+            def store(l, qkv):
+                k, v = qkv[:, d: 2 * d], qkv[:, 2 * d:]
+                ops.kv4_write(k, v, slots, s["cache"][l], values=(k, v))
+
+            self.forward(prompt, lm_head=False, on_qkv=store)
+            # LM head on each sequence's last position: row b*T0 + len-1 of the
+            # final LN, gathered as embeddings are
+            torch.sub(s["prompt_len"], 1, out=s["pos"])
+            rows = s["pos"] + torch.arange(0, B * T0, T0, dtype=torch.int32, device=self.device)
+            zero = torch.zeros(1, d, device=self.device)
+            check(lib().dc_embedding_fwd(rows.data_ptr(), self._bufs["af"].data_ptr(), zero.data_ptr(),
+                                         s["a"].data_ptr(), B, 1, d, B * T0, st), "dc_embedding_fwd")
+            last = s["a"]
+        else:
+            self.forward(prompt, lm_head=False)
+            b = self._bufs
+            for l in range(c.n_layers):
+                check(lib().dc_kv_cache_fill(b["qkv"][l].data_ptr(), 3 * d, B, T0, d, s["cache"][l].data_ptr(), st),
+                      "dc_kv_cache_fill")
+            # LM head on the last position only: rows b*T0 + T0-1 of the final LN
+            last = b["af"].view(B, T0, d)[:, T0 - 1, :]
         ops.gemm(last, P["wlm"][:, :V], out=s["logits"], bias=P["blm"])
         check(lib().dc_copy2d(s["tokens"].data_ptr(), Tm * 4, prompt.data_ptr(), T0 * 4, T0 * 4, B, st), "dc_copy2d")
-        s["pos"].fill_(T0 - 1)
+        if cache_bits != 4:
+            s["pos"].fill_(T0 - 1)
         self._greedy(s)
 
     def _greedy(self, s):
         c, P = self.cfg, self.P
+        if s["controls"] is not None:
+            ops.logits_controls(s["logits"], s["tokens"], s["pos"], prompt_len=s["prompt_len"], out=s["logits"],
+                                **s["controls"])
+        if s["key"][1] == 4:
+            ops.greedy_embed_rows(s["logits"], s["tokens"], s["pos"], wte=P["wte"], wpe=P["wpe"], x=s["x"])
+            return
         check(lib().dc_greedy_embed(s["logits"].data_ptr(), c.vocab, s["B"], c.vocab, P["wte"].data_ptr(),
                                     P["wpe"].data_ptr(), s["pos"].data_ptr(), c.d_model, s["tokens"].data_ptr(),
                                     c.block_size, s["x"].data_ptr(), ops._stream()), "dc_greedy_embed")
 
+    def _attend(self, s, l):
+        """Layer l's decode attention: append the step's k, v and attend."""
+        c = self.cfg
+        d, hs, Tm = c.d_model, c.head, c.block_size
+        if s["key"][1] == 4:
+            ops.aft_decode4(s["qkv"], s["w"][l], s["cache"][l], s["table"], s["pos"], s["ws"], out=s["zd"])
+            return
+        check(lib().dc_aft_decode(s["qkv"].data_ptr(), 3 * d, self.P[f"{l}.pos"].data_ptr(), Tm, Tm * Tm,
+                                  s["cache"][l].data_ptr(), s["B"], c.n_heads, hs, s["pos"].data_ptr(), Tm,
+                                  s["zd"].data_ptr(), d, s["ws"].data_ptr(), s["ws_bytes"], ops._stream()),
+              "dc_aft_decode")
+
     def decode_step(self):
         """Consume the token at position t = pos (its embedding is in s['x']),
-        append its k/v to every layer's history, emit the token of t+1."""
+        append its k/v to every layer's history, emit the token of t+1.  With
+        a 4-bit history every sequence has a position of its own, and one
+        whose position is set to -1 is left out of further steps."""
         c, P = self.cfg, self.P
         s = self._dec
-        B = s["B"]
-        d, hs, Tm = c.d_model, c.head, c.block_size
-        st = ops._stream()
         x = s["x"]
+        if s["key"][1] == 4:  # the page of the new position, for all layers
+            ops.page_tables(s["pos"], s["one"], s["free"], s["head"], s["table"], s["page_size"])
         for l in range(c.n_layers):
             ops.layernorm_fwd(x, P[f"{l}.ln1g"], P[f"{l}.ln1b"], out=s["a"])
             ops.gemm(s["a"], P[f"{l}.wqkv"], out=s["qkv"], bias=P[f"{l}.bqkv"])
-            check(lib().dc_aft_decode(s["qkv"].data_ptr(), 3 * d, P[f"{l}.pos"].data_ptr(), Tm, Tm * Tm,
-                                      s["cache"][l].data_ptr(), B, c.n_heads, hs, s["pos"].data_ptr(), Tm,
-                                      s["zd"].data_ptr(), d, s["ws"].data_ptr(), s["ws_bytes"], st), "dc_aft_decode")
+            self._attend(s, l)
             # residual adds in place on x (the step keeps no activations), so a
             # split-K GEMM starts from x itself rather than from a copy
             ops.gemm(s["zd"], P[f"{l}.wo"], out=x, bias=P[f"{l}.bo"], residual=x)
@@ -560,14 +674,18 @@ class AftDecoder:
         ops.gemm(s["a"], P["wlm"][:, : c.vocab], out=s["logits"], bias=P["blm"])
         self._greedy(s)
 
-    def generate(self, prompt: torch.Tensor, n_new: int, graph: bool = True):
+    def generate(self, prompt: torch.Tensor, n_new: int, graph: bool = True, lens=None, cache_bits: int = 32,
+                 page_size: int = 16, controls: LogitControls | None = None):
         """Greedy continuation of prompt [B, T0]: tokens [B, T0 + n_new].
         With ``graph`` the decode step is captured once as a CUDA graph and
-        replayed (the position advances on the device)."""
+        replayed (the position advances on the device).  ``lens``,
+        ``cache_bits`` and ``page_size`` as in ``prefill``: with lens,
+        sequence b's tokens are the first lens[b] + n_new of its row.
+        ``controls`` act on the logits before each pick."""
         B, T0 = prompt.shape
-        if T0 + n_new > self.cfg.block_size:
+        if (T0 if lens is None else max(int(n) for n in lens)) + n_new > self.cfg.block_size:
             raise ValueError("prompt + new tokens exceed the block size")
-        self.prefill(prompt)
+        self.prefill(prompt, lens=lens, cache_bits=cache_bits, n_new=n_new, page_size=page_size, controls=controls)
         steps = n_new - 1
         if steps > 0:
             self.decode_step()  # eager first step: one-time library setup happens here
@@ -586,4 +704,5 @@ class AftDecoder:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.decode_step()
+        g.decode_state = dict(self._dec)  # the buffers it replays on live as long as it
         return g
