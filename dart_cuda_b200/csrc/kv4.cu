@@ -90,10 +90,24 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16 *p, const fl
     *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
+template <typename T>
+__device__ __forceinline__ float to_f(T x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
 // One group's quantisation by the 4 lanes (xor 1, 2) that hold its 32 values:
 // step and low (bf16 values, the same on the 4 lanes), this lane's 8 codes.
-// All 32 lanes of the warp take part.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, float &low)
+// `lanes`: the lanes that take part, whole groups.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, float &low,
+                                              uint32_t lanes = 0xffffffffu)
 {
     float mn = x[0], mx = x[0];
     int bad = 0;
@@ -105,9 +119,9 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, 
     }
 #pragma unroll
     for (int o = 1; o <= 2; o *= 2) {
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+        mn = fminf(mn, __shfl_xor_sync(lanes, mn, o));
+        mx = fmaxf(mx, __shfl_xor_sync(lanes, mx, o));
+        bad |= __shfl_xor_sync(lanes, bad, o);
     }
     if (bad) {
         step = __uint_as_float(0x7fff0000u);
@@ -220,12 +234,23 @@ struct Decode {
     int64_t ldtab;
     const int32_t *pos;
     int B, D, hs, W, nslab, n_pages, page_size, cap;
+    int shift;  // page_size = 1 << shift
+    int w4;  // w's rows start on 16-byte boundaries
     void *Z;
     int64_t ldz;
     int *status;
+    int *counter;  // [B * nslab], zero between launches
+    float *part;   // [gridDim.x][2][3][W]
 };
 
 __device__ __forceinline__ float sigm(float q) { return 1.0f / (1.0f + __expf(-q)); }
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 // Larger of two, NaN if either is: a NaN in the history reaches Z.
 __device__ __forceinline__ float fmax_nan(float a, float b)
@@ -235,119 +260,316 @@ __device__ __forceinline__ float fmax_nan(float a, float b)
     return r;
 }
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 4;
+constexpr int kRows = 8;  // history rows of a block: never split over pages
 
-// One block per (sequence, slab).  A row's W channels are W/8 lanes, so a
-// warp reads 256/W rows at once; the warps' running (max, num, den) per
-// channel meet in shared memory.
+// Blocks of kRows rows that position t's history has; 0: inactive.
+__device__ __forceinline__ int row_blocks(const Decode &p, int t)
+{
+    return t < 0 || t >= p.cap ? 0 : t / kRows + 1;
+}
+
+__device__ __forceinline__ void join(float &m, float &num, float &den, float m2, float num2, float den2)
+{
+    const float mx = fmax_nan(m, m2);
+    if (mx == -INFINITY) return;
+    const float a = ex2(m - mx), c = ex2(m2 - mx);
+    num = num * a + num2 * c;
+    den = den * a + den2 * c;
+    m = mx;
+}
+
+// The history of a slab (W channels of one sequence) is read once, in blocks
+// of kRows rows by W/8 lanes of 8 channels each; exponents are in base 2
+// (k and w scaled by log2 e), and each channel keeps (ref, num, den) with
+// num, den = sums of 2^(y - ref) v and 2^(y - ref) in fp32.
+//
+// Work split: the row blocks of all (sequence, slab) items, one after the
+// other, are cut into equal shares of q blocks, one share a CTA, so ragged
+// lengths balance and a long sequence spreads over many CTAs.  An item that
+// several CTAs share is merged, in CTA order, by the last of them to finish.
 template <typename T, int LPR>
-__global__ void __launch_bounds__(32 * kWarps) decode_kernel(Decode p)
+__global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
-    constexpr int RPW = 32 / LPR;
-    const int b = blockIdx.x / p.nslab, slab = blockIdx.x % p.nslab;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int RPW = 32 / LPR;       // row blocks a warp reads at once
+    constexpr int W = LPR * 8;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int sub = lane / LPR, oct = lane % LPR;
-    const int ch = slab * p.W + oct * 8;
-    T *z = static_cast<T *>(p.Z) + b * p.ldz + ch;
-    const int t = p.pos[b];
-    const float zero[8] = {};
-    if (t < 0 || t >= p.cap) {  // an inactive row
-        if (t >= 0 && threadIdx.x == 0) atomicOr(p.status, DC_DEVERR_FULL);
-        if (threadIdx.x < LPR) store8(z, zero);
-        return;
-    }
-    const int32_t *tab = p.table + b * p.ldtab;
-    const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + ch;
-    if (warp == 0) {  // append position t
-        float k[8], v[8], ks, kl, vs, vl;
-        load8(row + p.D, k);
-        load8(row + 2 * p.D, v);
-        const uint32_t kc = quantise8(k, ks, kl), vc = quantise8(v, vs, vl);
-        const int page = tab[t / p.page_size];
-        if (page < 0 || page >= p.n_pages) {
-            if (lane == 0) atomicOr(p.status, DC_DEVERR_PAGE);
-        } else if (sub == 0) {
-            uint8_t *rec = p.pages + record(page, t % p.page_size, slab, p.nslab, p.page_size, p.W);
-            *reinterpret_cast<uint2 *>(rec + oct * 8) = make_uint2(kc, vc);
-            if (oct % 4 == 0)
-                *reinterpret_cast<uint2 *>(rec + p.W + oct * 2) =
-                    make_uint2(pack_params(ks, kl), pack_params(vs, vl));
+    __shared__ float part[kWarps][3][W];
+    __shared__ int s_sum[kWarps], s_max[kWarps], s_b, s_first, s_last;
+
+    // this CTA's share [u, u1) of the row blocks
+    int sum = 0, most = 0;
+    for (int b = tid; b < p.B; b += kThreads) {
+        const int t = p.pos[b], nb = row_blocks(p, t);
+        sum += nb;
+        most = max(most, nb);
+        if (nb == 0 && b % gridDim.x == blockIdx.x) {  // an inactive sequence
+            if (t >= 0) atomicOr(p.status, DC_DEVERR_FULL);
+            const float zero[8] = {};
+            for (int c = 0; c < p.D; c += 8) store8(static_cast<T *>(p.Z) + b * p.ldz + c, zero);
         }
+    }
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+        s_sum[warp] = sum;
+        s_max[warp] = most;
     }
     __syncthreads();
-    const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
-    float m[8], num[8], den[8];
+    sum = most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        m[j] = -INFINITY;
-        num[j] = den[j] = 0.f;
+    for (int k = 0; k < kWarps; ++k) {
+        sum += s_sum[k];
+        most = max(most, s_max[k]);
     }
-    for (int i = warp * RPW + sub; i <= t; i += kWarps * RPW) {
-        const int page = tab[i / p.page_size];
-        if (page < 0 || page >= p.n_pages) {
-            if (oct == 0) atomicOr(p.status, DC_DEVERR_PAGE);
-            continue;
+    const int64_t total = (int64_t)sum * p.nslab;
+    const int q = (int)max((total + gridDim.x - 1) / gridDim.x, (int64_t)sqrtf((float)most) + 1);
+    int64_t u = (int64_t)blockIdx.x * q;
+    const int64_t u1 = min(total, u + q);
+    if (u >= u1) return;
+    // the sequence that unit u lies in: blocks before it, over all sequences
+    const int target = (int)(u / p.nslab);
+    int before = 0;
+    for (int b0 = 0;; b0 += kThreads) {
+        const int b = b0 + tid;
+        const int nb = b < p.B ? row_blocks(p, p.pos[b]) : 0;
+        int inc = nb;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
         }
-        const uint8_t *rec = p.pages + record(page, i % p.page_size, slab, p.nslab, p.page_size, p.W);
-        const uint2 code = *reinterpret_cast<const uint2 *>(rec + oct * 8);
-        const uint2 par = *reinterpret_cast<const uint2 *>(rec + p.W + oct / 4 * 8);
-        const float wi = w[i];
-        float k[8], v[8];
-        values8(code.x, par.x, k);
-        values8(code.y, par.y, v);
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = inc;
+        if (tid == 0) s_b = -1;
+        __syncthreads();
+        int at = before, all = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+            if (k < warp) at += s_sum[k];
+            all += s_sum[k];
+        }
+        if (nb && target >= at + inc - nb && target < at + inc) {
+            s_b = b;
+            s_first = at + inc - nb;
+        }
+        __syncthreads();
+        before += all;
+        if (s_b >= 0) break;  // total > target: some sequence holds it
+    }
+    int b = s_b;
+    int t = p.pos[b], nb = row_blocks(p, t);
+    int slab = (int)((u - (int64_t)s_first * p.nslab) / nb);
+    int blk = (int)((u - (int64_t)s_first * p.nslab) % nb);
+
+    for (bool first = true;; first = false) {
+        const int n = (int)min((int64_t)(nb - blk), u1 - u);
+        const int ch = slab * W + oct * 8;
+        const int32_t *tab = p.table + b * p.ldtab;
+        const T *row = static_cast<const T *>(p.qkv) + b * p.ldq;
+        const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
+        float ref[8], num[8], den[8], low = -INFINITY;  // low: the smallest ref, -inf while one is unset
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ref[j] = num[j] = den[j] = 0.f;
+        for (int k = warp * RPW + sub; k < n; k += kWarps * RPW) {
+            const int i0 = (blk + k) * kRows;
+            const int page = tab[i0 >> p.shift];
+            const bool ok = page >= 0 && page < p.n_pages;
+            if (!ok && oct == 0) atomicOr(p.status, DC_DEVERR_PAGE);
+            const int rows = ok ? min(kRows, t - i0) : 0;  // rows stored before this call
+            uint8_t *rec = p.pages + record(ok ? page : 0, i0 & (p.page_size - 1), slab, p.nslab, p.page_size, W);
+            uint2 code[kRows], par[kRows];
+            float wl[kRows];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                code[r] = par[r] = make_uint2(0, 0);
+                if (r < rows) {
+                    code[r] = *reinterpret_cast<const uint2 *>(rec + r * (W * 5 / 4) + oct * 8);
+                    par[r] = *reinterpret_cast<const uint2 *>(rec + r * (W * 5 / 4) + W + oct / 4 * 8);
+                }
+            }
+            if (rows == kRows && p.w4) {
+                const float4 a = *reinterpret_cast<const float4 *>(w + i0), c = *reinterpret_cast<const float4 *>(w + i0 + 4);
+                wl[0] = a.x; wl[1] = a.y; wl[2] = a.z; wl[3] = a.w;
+                wl[4] = c.x; wl[5] = c.y; wl[6] = c.z; wl[7] = c.w;
+            } else {
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) wl[r] = r < rows || (ok && i0 + r == t) ? w[i0 + r] : -INFINITY;
+            }
+            if (rows < kRows && ok) {  // position t itself: quantise and append
+                float x[8], st, lo;
+                const uint32_t lanes = 0xfu << (lane & ~3);
+                uint2 c, pr;
+                load8(row + p.D + ch, x);
+                c.x = quantise8(x, st, lo, lanes);
+                pr.x = pack_params(st, lo);
+                load8(row + 2 * p.D + ch, x);
+                c.y = quantise8(x, st, lo, lanes);
+                pr.y = pack_params(st, lo);
+                *reinterpret_cast<uint2 *>(rec + rows * (W * 5 / 4) + oct * 8) = c;
+                if (oct % 4 == 0) *reinterpret_cast<uint2 *>(rec + rows * (W * 5 / 4) + W + oct * 2) = pr;
+#pragma unroll
+                for (int r = 0; r < kRows; ++r)
+                    if (r == rows) {
+                        code[r] = c;
+                        par[r] = pr;
+                    }
+            }
+            // y = log2(e) (low + step c + w) = a + s (1 + c/16), with the code
+            // put into a mantissa's top bits; top: a bound on the block's y
+            float ks[kRows], ka[kRows], top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const float step16 = 16.f * __uint_as_float(par[r].x << 16);
+                wl[r] *= kLog2e;
+                ks[r] = step16 * kLog2e;
+                ka[r] = fmaf(__uint_as_float(par[r].x & 0xffff0000u) - step16, kLog2e, wl[r]);
+                top = fmax_nan(top, fmaf(ks[r], 1.9375f, ka[r]));
+            }
+            auto y = [&](int r, int j) {
+                const uint32_t c = j < 5 ? code[r].x << (19 - 4 * j) : code[r].x >> (4 * j - 19);
+                return fmaf(ks[r], __uint_as_float((c & 0x780000u) | 0x3f800000u), ka[r]);
+            };
+            // terms up to 2^16 above a channel's ref are summed as they are;
+            // else the refs rise to the largest exponents so far.  (Exponents
+            // beyond the range of fp32 in base 2, as of a bias of -FLT_MAX,
+            // count as its end.)
+            if (!(low > -1e30f && top <= low + 16.f)) {
+#pragma unroll
+                for (int r = 0; r < kRows; ++r)
+                    if (isinf(wl[r]) && ok && (r < rows || i0 + r == t) && !isinf(w[i0 + r]))
+                        ka[r] = copysignf(3.4028234e38f, wl[r]);
+                low = INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float old = den[j] == 0.f ? -INFINITY : ref[j];
+                    float mx = old;
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) mx = fmax_nan(mx, y(r, j));
+                    low = fminf(low, mx);
+                    if (mx == -INFINITY) continue;
+                    const float scale = ex2(old - mx);
+                    num[j] *= scale;
+                    den[j] *= scale;
+                    ref[j] = mx;
+                }
+            }
+            float va[kRows], vs[kRows];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                vs[r] = 16.f * __uint_as_float(par[r].y << 16);
+                va[r] = __uint_as_float(par[r].y & 0xffff0000u) - vs[r];
+            }
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float e = ex2(y(r, j) - ref[j]);
+                    const uint32_t c = j < 5 ? code[r].y << (19 - 4 * j) : code[r].y >> (4 * j - 19);
+                    const float v = fmaf(vs[r], __uint_as_float((c & 0x780000u) | 0x3f800000u), va[r]);
+                    num[j] = fmaf(e, v, num[j]);
+                    den[j] += e;
+                }
+        }
+        // blocks of a warp, then warps
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = k[j] + wi;
-            const float mx = fmax_nan(m[j], x);
-            if (mx == -INFINITY) continue;  // masked so far
-            const float scale = __expf(m[j] - mx), e = __expf(x - mx);
-            num[j] = num[j] * scale + e * v[j];
-            den[j] = den[j] * scale + e;
-            m[j] = mx;
+            if (den[j] == 0.f) ref[j] = -INFINITY;
+#pragma unroll
+            for (int o = LPR; o < 32; o *= 2) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, ref[j], o);
+                const float n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
+                const float d2 = __shfl_xor_sync(0xffffffffu, den[j], o);
+                join(ref[j], num[j], den[j], m2, n2, d2);
+            }
         }
+        if (sub == 0) {
+            store8(&part[warp][0][oct * 8], ref);
+            store8(&part[warp][1][oct * 8], num);
+            store8(&part[warp][2][oct * 8], den);
+        }
+        __syncthreads();
+        constexpr int CPT = (W + kThreads - 1) / kThreads;  // channels a thread finishes
+        float fm[CPT], fn[CPT], fd[CPT];
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int c = tid + k * kThreads;
+            if (c >= W) continue;
+            fm[k] = part[0][0][c];
+            fn[k] = part[0][1][c];
+            fd[k] = part[0][2][c];
+#pragma unroll
+            for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part[g][0][c], part[g][1][c], part[g][2][c]);
+        }
+        bool finish = n == nb;
+        if (!finish) {  // shared with other CTAs
+            float *mine = p.part + ((int64_t)blockIdx.x * 2 + !first) * 3 * W;
+#pragma unroll
+            for (int k = 0; k < CPT; ++k) {
+                const int c = tid + k * kThreads;
+                if (c >= W) continue;
+                mine[c] = fm[k];
+                mine[W + c] = fn[k];
+                mine[2 * W + c] = fd[k];
+            }
+            __threadfence();
+            __syncthreads();
+            const int64_t u_item = u - blk;
+            const int j0 = (int)(u_item / q), j1 = (int)((u_item + nb - 1) / q);
+            if (tid == 0) {
+                int *counter = p.counter + (int64_t)b * p.nslab + slab;
+                s_last = atomicAdd(counter, 1) == j1 - j0;
+                if (s_last) *counter = 0;  // ready for the next launch
+            }
+            __syncthreads();
+            if (s_last) {
+                finish = true;
+                __threadfence();
+#pragma unroll
+                for (int k = 0; k < CPT; ++k) {
+                    const int c = tid + k * kThreads;
+                    if (c >= W) continue;
+                    fm[k] = -INFINITY;
+                    fn[k] = fd[k] = 0.f;
+                    for (int g = j0; g <= j1; ++g) {
+                        // the item is CTA g's first unless it begins inside g's share
+                        const float *src = p.part + ((int64_t)g * 2 + (u_item > (int64_t)g * q)) * 3 * W + c;
+                        join(fm[k], fn[k], fd[k], __ldcg(src), __ldcg(src + W), __ldcg(src + 2 * W));
+                    }
+                }
+            }
+        }
+        if (finish) {
+#pragma unroll
+            for (int k = 0; k < CPT; ++k) {
+                const int c = tid + k * kThreads;
+                if (c >= W) continue;
+                const float qv = to_f<T>(row[slab * W + c]);
+                static_cast<T *>(p.Z)[b * p.ldz + slab * W + c] =
+                    from_f<T>(fd[k] == 0.f ? 0.f : sigm(qv) * (fn[k] / fd[k]));
+            }
+        }
+        u += n;
+        if (u >= u1) return;
+        blk = 0;
+        if (++slab == p.nslab) {
+            slab = 0;
+            do t = p.pos[++b];  // u < total: there is another active one
+            while ((nb = row_blocks(p, t)) == 0);
+        }
+        __syncthreads();  // part is reused
     }
-    // rows of a warp, then warps
-    auto join = [](float &m, float &num, float &den, float m2, float num2, float den2) {
-        const float mx = fmax_nan(m, m2);
-        if (mx == -INFINITY) return;
-        const float a = __expf(m - mx), c = __expf(m2 - mx);
-        num = num * a + num2 * c;
-        den = den * a + den2 * c;
-        m = mx;
-    };
-#pragma unroll
-    for (int o = LPR; o < 32; o *= 2)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            join(m[j], num[j], den[j], __shfl_xor_sync(0xffffffffu, m[j], o),
-                 __shfl_xor_sync(0xffffffffu, num[j], o), __shfl_xor_sync(0xffffffffu, den[j], o));
-    __shared__ float part[kWarps][3][8][LPR];
-    if (sub == 0)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            part[warp][0][j][oct] = m[j];
-            part[warp][1][j][oct] = num[j];
-            part[warp][2][j][oct] = den[j];
-        }
-    __syncthreads();
-    if (threadIdx.x >= LPR) return;
-    for (int k = 1; k < kWarps; ++k)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            join(m[j], num[j], den[j], part[k][0][j][oct], part[k][1][j][oct], part[k][2][j][oct]);
-    float q[8];
-    load8(row, q);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = den[j] == 0.f ? 0.f : sigm(q[j]) * (num[j] / den[j]);
-    store8(z, q);
 }
+
+static int decode_grid() { return kResident * sm_count(); }
 
 template <typename T>
 static cudaError_t launch_decode(const Decode &p, cudaStream_t st)
 {
-    const dim3 grid((unsigned)(p.B * p.nslab)), block(32 * kWarps);
+    const dim3 grid((unsigned)decode_grid()), block(kThreads);
     switch (p.W) {
         case 256: return launch_pdl(decode_kernel<T, 32>, grid, block, 0, st, 1, p);
         case 128: return launch_pdl(decode_kernel<T, 16>, grid, block, 0, st, 1, p);
@@ -427,8 +649,9 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
 
 size_t dc_aft_decode4_workspace_size(int B, int D)
 {
-    if (B <= 0 || D <= 0) return 0;
-    return 256;
+    const int W = D > 0 ? kv4::slab_width(D) : 0;
+    if (B <= 0 || !W) return 0;
+    return round_up((int64_t)B * (D / W) * sizeof(int), 256) + (size_t)kv4::decode_grid() * 2 * 3 * W * sizeof(float);
 }
 
 int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw, long long head_stride_w,
@@ -471,11 +694,17 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     p.n_pages = n_pages;
     p.page_size = page_size;
     p.cap = (int)std::min<int64_t>(Tmax, (int64_t)ldtab * page_size);
+    for (p.shift = 3; 1 << p.shift < page_size;) ++p.shift;
+    p.w4 = aligned16(w) && ldw % 4 == 0 && head_stride_w % 4 == 0;
+    p.counter = static_cast<int *>(workspace);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                       round_up((int64_t)B * p.nslab * sizeof(int), 256));
     p.Z = Z;
     p.ldz = ldz;
     p.status = device_status_word();
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
-    if ((int64_t)B * p.nslab > INT32_MAX) return fail(DC_ERR_INVALID, "B * D too large");
+    if ((int64_t)B * (p.cap / kRows + 1) > INT32_MAX || (int64_t)B * p.nslab > INT32_MAX / 4)
+        return fail(DC_ERR_INVALID, "B * Tmax or B * D too large");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("aft_decode4", st);
     DC_CUDA_TRY(dtype == DC_F32 ? launch_decode<float>(p, st) : launch_decode<__nv_bfloat16>(p, st));

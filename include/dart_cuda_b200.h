@@ -374,8 +374,8 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
  * pos >= min(Tmax, ldtab * page_size), which sets status bit 0x40, and one
  * whose bias row is -inf throughout.  Sequences may share pages they only
  * read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
- * zero-filled once before its first use (the kernel leaves it zeroed); calls
- * that may overlap on the GPU need one each. */
+ * zero-filled once before its first use (the kernel leaves its counters
+ * zeroed); calls that may overlap on the GPU need one each. */
 size_t dc_aft_decode4_workspace_size(int B, int D);
 int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
                    long long head_stride_w, void *pages, int n_pages, int page_size,

@@ -268,7 +268,7 @@ class History:
         assert np.array_equal(np.isnan(g), np.isnan(z))
         bad = ~(np.abs(g - z) <= tol) & ~np.isnan(z)
         assert not bad.any(), (np.abs(g - z)[bad].max(), np.argwhere(bad)[:4])
-        assert torch.count_nonzero(self.ws) == 0
+        assert torch.count_nonzero(self.ws[: 4 * self.B * (self.D // ref.slab(self.D))]) == 0  # counters left at zero
         again = self.step()  # idempotent, the same bits
         assert self.ops.read_status() == status
         assert torch.equal(torch.nan_to_num(again, 7.0), torch.nan_to_num(got, 7.0))
