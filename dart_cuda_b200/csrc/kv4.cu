@@ -164,6 +164,37 @@ __device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (
     for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
 }
 
+// d = a * b + c with bf16 factors in the low halves of a and b, c in fp32.
+__device__ __forceinline__ float fma_bf16(uint32_t a, uint32_t b, float c)
+{
+    float d;
+    asm("{\n\t.reg .b16 a, b;\n\tcvt.u16.u32 a, %1;\n\tcvt.u16.u32 b, %2;\n\t"
+        "fma.rn.f32.bf16 %0, a, b, %3;\n\t}\n"
+        : "=f"(d)
+        : "r"(a), "r"(b), "f"(c));
+    return d;
+}
+
+// low - 128 step of a pair of parameters (exact unless low is negligible or
+// 2^15 times step), and from it the values of codes j and j + 4: a code in
+// the low mantissa bits of the bf16 128 is the bf16 number 128 + code, so one
+// mask makes the factors of two values.
+__device__ __forceinline__ float base128(uint32_t params)
+{
+    return fma_bf16(0xc300, params, __uint_as_float(params & 0xffff0000u));
+}
+__device__ __forceinline__ float2 value2(uint32_t codes, int j, uint32_t params, float base)
+{
+    uint32_t c;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(c) : "r"(codes >> (4 * j)));
+    float2 x;
+    asm("{\n\t.reg .b16 a, b, s, u;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 {s, u}, %3;\n\t"
+        "fma.rn.f32.bf16 %0, a, s, %4;\n\tfma.rn.f32.bf16 %1, b, s, %4;\n\t}\n"
+        : "=f"(x.x), "=f"(x.y)
+        : "r"(c), "r"(params), "f"(base));
+    return x;
+}
+
 // Byte offset of the record of slab `slab` at slot (page, row).
 __device__ __forceinline__ size_t record(int page, int row, int slab, int nslab, int page_size, int W)
 {
@@ -371,9 +402,11 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
         const int32_t *tab = p.table + b * p.ldtab;
         const T *row = static_cast<const T *>(p.qkv) + b * p.ldq;
         const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
-        float ref[8], num[8], den[8], low = -INFINITY;  // low: the smallest ref, -inf while one is unset
+        // channels j and j + 4 of the lane's 8 in pairs
+        float2 ref[4], num[4], den[4];
+        float low = -INFINITY;  // the smallest ref, -inf while one is unset
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ref[j] = num[j] = den[j] = 0.f;
+        for (int j = 0; j < 4; ++j) ref[j] = num[j] = den[j] = make_float2(0.f, 0.f);
         for (int k = warp * RPW + sub; k < n; k += kWarps * RPW) {
             const int i0 = (blk + k) * kRows;
             const int page = tab[i0 >> p.shift];
@@ -418,21 +451,15 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
                         par[r] = pr;
                     }
             }
-            // y = log2(e) (low + step c + w) = a + s (1 + c/16), with the code
-            // put into a mantissa's top bits; top: a bound on the block's y
-            float ks[kRows], ka[kRows], top = -INFINITY;
+            // y = log2(e) (k + w), k = low + step * code
+            float ka[kRows], va[kRows], top = -INFINITY;  // top: a bound on the block's y
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
-                const float step16 = 16.f * __uint_as_float(par[r].x << 16);
                 wl[r] *= kLog2e;
-                ks[r] = step16 * kLog2e;
-                ka[r] = fmaf(__uint_as_float(par[r].x & 0xffff0000u) - step16, kLog2e, wl[r]);
-                top = fmax_nan(top, fmaf(ks[r], 1.9375f, ka[r]));
+                ka[r] = base128(par[r].x);
+                va[r] = base128(par[r].y);
+                top = fmax_nan(top, fmaf(fma_bf16(0x430f, par[r].x, ka[r]), kLog2e, wl[r]));
             }
-            auto y = [&](int r, int j) {
-                const uint32_t c = j < 5 ? code[r].x << (19 - 4 * j) : code[r].x >> (4 * j - 19);
-                return fmaf(ks[r], __uint_as_float((c & 0x780000u) | 0x3f800000u), ka[r]);
-            };
             // terms up to 2^16 above a channel's ref are summed as they are;
             // else the refs rise to the largest exponents so far.  (Exponents
             // beyond the range of fp32 in base 2, as of a bias of -FLT_MAX,
@@ -441,55 +468,63 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
 #pragma unroll
                 for (int r = 0; r < kRows; ++r)
                     if (isinf(wl[r]) && ok && (r < rows || i0 + r == t) && !isinf(w[i0 + r]))
-                        ka[r] = copysignf(3.4028234e38f, wl[r]);
+                        wl[r] = copysignf(3.4028234e38f, wl[r]);
                 low = INFINITY;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float old = den[j] == 0.f ? -INFINITY : ref[j];
-                    float mx = old;
+                for (int j = 0; j < 4; ++j) {
+                    float2 mx, old;
+                    old.x = mx.x = den[j].x == 0.f ? -INFINITY : ref[j].x;
+                    old.y = mx.y = den[j].y == 0.f ? -INFINITY : ref[j].y;
 #pragma unroll
-                    for (int r = 0; r < kRows; ++r) mx = fmax_nan(mx, y(r, j));
-                    low = fminf(low, mx);
-                    if (mx == -INFINITY) continue;
-                    const float scale = ex2(old - mx);
-                    num[j] *= scale;
-                    den[j] *= scale;
-                    ref[j] = mx;
+                    for (int r = 0; r < kRows; ++r) {
+                        const float2 y = __ffma2_rn(value2(code[r].x, j, par[r].x, ka[r]),
+                                                    make_float2(kLog2e, kLog2e), make_float2(wl[r], wl[r]));
+                        mx.x = fmax_nan(mx.x, y.x);
+                        mx.y = fmax_nan(mx.y, y.y);
+                    }
+                    low = fminf(low, fminf(mx.x, mx.y));
+                    auto raise = [](float mx, float old, float &ref, float &num, float &den) {
+                        if (mx == -INFINITY) return;
+                        const float scale = ex2(old - mx);
+                        num *= scale;
+                        den *= scale;
+                        ref = mx;
+                    };
+                    raise(mx.x, old.x, ref[j].x, num[j].x, den[j].x);
+                    raise(mx.y, old.y, ref[j].y, num[j].y, den[j].y);
                 }
-            }
-            float va[kRows], vs[kRows];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                vs[r] = 16.f * __uint_as_float(par[r].y << 16);
-                va[r] = __uint_as_float(par[r].y & 0xffff0000u) - vs[r];
             }
 #pragma unroll
             for (int r = 0; r < kRows; ++r)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float e = ex2(y(r, j) - ref[j]);
-                    const uint32_t c = j < 5 ? code[r].y << (19 - 4 * j) : code[r].y >> (4 * j - 19);
-                    const float v = fmaf(vs[r], __uint_as_float((c & 0x780000u) | 0x3f800000u), va[r]);
-                    num[j] = fmaf(e, v, num[j]);
-                    den[j] += e;
+                for (int j = 0; j < 4; ++j) {
+                    float2 y = __ffma2_rn(value2(code[r].x, j, par[r].x, ka[r]), make_float2(kLog2e, kLog2e),
+                                          make_float2(wl[r], wl[r]));
+                    y = __fadd2_rn(y, make_float2(-ref[j].x, -ref[j].y));
+                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                    num[j] = __ffma2_rn(e, value2(code[r].y, j, par[r].y, va[r]), num[j]);
+                    den[j] = __fadd2_rn(den[j], e);
                 }
         }
         // blocks of a warp, then warps
+        float fr[8], fu[8], fe[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (den[j] == 0.f) ref[j] = -INFINITY;
+            fe[j] = j < 4 ? den[j & 3].x : den[j & 3].y;
+            fu[j] = j < 4 ? num[j & 3].x : num[j & 3].y;
+            fr[j] = fe[j] == 0.f ? -INFINITY : j < 4 ? ref[j & 3].x : ref[j & 3].y;
 #pragma unroll
             for (int o = LPR; o < 32; o *= 2) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, ref[j], o);
-                const float n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
-                const float d2 = __shfl_xor_sync(0xffffffffu, den[j], o);
-                join(ref[j], num[j], den[j], m2, n2, d2);
+                const float m2 = __shfl_xor_sync(0xffffffffu, fr[j], o);
+                const float n2 = __shfl_xor_sync(0xffffffffu, fu[j], o);
+                const float d2 = __shfl_xor_sync(0xffffffffu, fe[j], o);
+                join(fr[j], fu[j], fe[j], m2, n2, d2);
             }
         }
         if (sub == 0) {
-            store8(&part[warp][0][oct * 8], ref);
-            store8(&part[warp][1][oct * 8], num);
-            store8(&part[warp][2][oct * 8], den);
+            store8(&part[warp][0][oct * 8], fr);
+            store8(&part[warp][1][oct * 8], fu);
+            store8(&part[warp][2][oct * 8], fe);
         }
         __syncthreads();
         constexpr int CPT = (W + kThreads - 1) / kThreads;  // channels a thread finishes
