@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "dc_internal.h"
 #include "dc_ptx.cuh"
@@ -137,18 +138,30 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, 
         step = 0.f;
         return 0;
     }
-    uint32_t codes = 0;
+    // (x - low) / step, rounded: off by at most 2^-22 of its value (tiny steps
+    // are scaled first), so the nearest whole number is the code unless that
+    // lies 0.5 away to within 1e-5; there the borders decide
+    const float scale = step < 1e-30f ? 0x1p100f : 1.f, inv = __frcp_rn(step * scale);
+    float c[8], worst = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float c = fminf(fmaxf(floorf(__fdiv_rn(x[j] - low, step) + 0.5f), 0.f), 15.f);
-        // the estimate is within one of the code; the borders decide
-        if (c > 0.f && x[j] < __fmaf_ru(step, c - 0.5f, low))
-            c -= 1.f;
-        else if (c < 15.f && x[j] >= __fmaf_ru(step, c + 0.5f, low))
-            c += 1.f;
-        codes |= (uint32_t)c << (4 * j);
+        const float q = (x[j] - low) * scale * inv;
+        c[j] = (q + 12582912.f) - 12582912.f;
+        worst = fmaxf(worst, fabsf(q - c[j]));
     }
-    return codes;
+    if (worst > 0.49999f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (x[j] < __fmaf_ru(step, c[j] - 0.5f, low))
+                c[j] -= 1.f;
+            else if (x[j] >= __fmaf_ru(step, c[j] + 0.5f, low))
+                c[j] += 1.f;
+        }
+    }
+    // four codes are the digits of a number below 2^16
+    const float lo4 = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
+    const float hi4 = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
+    return __byte_perm(__float_as_uint(lo4), __float_as_uint(hi4), 0x5410);
 }
 
 __device__ __forceinline__ uint32_t pack_params(float step, float low)
@@ -164,38 +177,53 @@ __device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (
     for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
 }
 
-// d = a * b + c with bf16 factors in the low halves of a and b, c in fp32.
-__device__ __forceinline__ float fma_bf16(uint32_t a, uint32_t b, float c)
+// Pairs of fp32 numbers in a 64-bit register (the type that keeps a pair of
+// equal numbers in place: float2 operands were copied at every use).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y)
 {
-    float d;
-    asm("{\n\t.reg .b16 a, b;\n\tcvt.u16.u32 a, %1;\n\tcvt.u16.u32 b, %2;\n\t"
-        "fma.rn.f32.bf16 %0, a, b, %3;\n\t}\n"
-        : "=f"(d)
-        : "r"(a), "r"(b), "f"(c));
-    return d;
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 a)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
-// low - 128 step of a pair of parameters (exact unless low is negligible or
-// 2^15 times step), and from it the values of codes j and j + 4: a code in
-// the low mantissa bits of the bf16 128 is the bf16 number 128 + code, so one
-// mask makes the factors of two values.
-__device__ __forceinline__ float base128(uint32_t params)
+// Two codes as fp32 numbers 1/2 + c/32: the codes of a word are masked into
+// bits 3..6 of its bytes (8 codes: two words, of even and odd channels), and
+// a byte becomes the top of a mantissa by one byte permutation.  Pair j holds
+// channels 0, 2 | 4, 6 | 1, 3 | 5, 7.
+__device__ __forceinline__ f32x2 factors(uint32_t even, uint32_t odd, int j)
 {
-    return fma_bf16(0xc300, params, __uint_as_float(params & 0xffff0000u));
-}
-__device__ __forceinline__ float2 value2(uint32_t codes, int j, uint32_t params, float base)
-{
-    uint32_t c;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(c) : "r"(codes >> (4 * j)));
-    float2 x;
-    asm("{\n\t.reg .b16 a, b, s, u;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 {s, u}, %3;\n\t"
-        "fma.rn.f32.bf16 %0, a, s, %4;\n\tfma.rn.f32.bf16 %1, b, s, %4;\n\t}\n"
-        : "=f"(x.x), "=f"(x.y)
-        : "r"(c), "r"(params), "f"(base));
-    return x;
+    const uint32_t w = j < 2 ? even : odd;
+    const uint32_t k = 2 * (j & 1);
+    return pack2(__uint_as_float(__byte_perm(w, 0x3f000000u, 0x7044u | k << 8)),
+                 __uint_as_float(__byte_perm(w, 0x3f000000u, 0x7044u | (k + 1) << 8)));
 }
 
-// Byte offset of the record of slab `slab` at slot (page, row).
+// Byte offset of the record// Byte offset of the record of slab `slab` at slot (page, row).
 __device__ __forceinline__ size_t record(int page, int row, int slab, int nslab, int page_size, int W)
 {
     return (((size_t)page * nslab + slab) * page_size + row) * (size_t)(W * 5 / 4);
@@ -265,6 +293,7 @@ struct Decode {
     int64_t ldtab;
     const int32_t *pos;
     int B, D, hs, W, nslab, n_pages, page_size, cap;
+    uint32_t page_bytes;
     int shift;  // page_size = 1 << shift
     int w4;  // w's rows start on 16-byte boundaries
     void *Z;
@@ -291,8 +320,21 @@ __device__ __forceinline__ float fmax_nan(float a, float b)
     return r;
 }
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 4;
-constexpr int kRows = 8;  // history rows of a block: never split over pages
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 3;
+constexpr int kRows = 16;  // history rows of a block: two halves, each within a page
+constexpr int kStages = 3;  // blocks in flight of a warp
+
+// 16 bytes, of which the first `bytes` (0 or 16) are read, the others zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 // Blocks of kRows rows that position t's history has; 0: inactive.
 __device__ __forceinline__ int row_blocks(const Decode &p, int t)
@@ -310,31 +352,119 @@ __device__ __forceinline__ void join(float &m, float &num, float &den, float m2,
     m = mx;
 }
 
+// The sums of one item with a running maximum per channel, by the whole CTA,
+// from the stored history (position t appended): num [W], den [W] into out.
+// out holds 3 * W * kWarps floats.
+template <int W>
+__device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, float *out)
+{
+    constexpr int LPR = W / 8, RPW = 32 / LPR;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPR, oct = lane % LPR;
+    const int ch = slab * W + oct * 8;
+    const int32_t *tab = p.table + b * p.ldtab;
+    const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
+    float m[8], num[8], den[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        m[j] = -INFINITY;
+        num[j] = den[j] = 0.f;
+    }
+    for (int i = warp * RPW + sub; i <= t; i += kWarps * RPW) {
+        const int page = tab[i >> p.shift];
+        if (page < 0 || page >= p.n_pages) continue;
+        const uint8_t *rec = p.pages + record(page, i & (p.page_size - 1), slab, p.nslab, p.page_size, W);
+        const uint2 code = *reinterpret_cast<const uint2 *>(rec + oct * 8);
+        const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + oct / 4 * 8);
+        const float wi = w[i];
+        float k[8], v[8];
+        values8(code.x, par.x, k);
+        values8(code.y, par.y, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = k[j] + wi;
+            const float mx = fmax_nan(m[j], x);
+            if (mx == -INFINITY) continue;  // masked so far
+            const float scale = ex2((m[j] - mx) * kLog2e), e = ex2((x - mx) * kLog2e);
+            num[j] = num[j] * scale + e * v[j];
+            den[j] = den[j] * scale + e;
+            m[j] = mx;
+        }
+    }
+    auto add = [](float &m, float &num, float &den, float m2, float num2, float den2) {
+        const float mx = fmax_nan(m, m2);
+        if (mx == -INFINITY) return;
+        const float a = ex2((m - mx) * kLog2e), c = ex2((m2 - mx) * kLog2e);
+        num = num * a + num2 * c;
+        den = den * a + den2 * c;
+        m = mx;
+    };
+#pragma unroll
+    for (int o = LPR; o < 32; o *= 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o), n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
+            add(m[j], num[j], den[j], m2, n2, __shfl_xor_sync(0xffffffffu, den[j], o));
+        }
+    __syncthreads();
+    if (sub == 0) {
+        store8(out + (warp * 3 + 0) * W + oct * 8, num);
+        store8(out + (warp * 3 + 1) * W + oct * 8, den);
+        store8(out + (warp * 3 + 2) * W + oct * 8, m);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < W; c += kThreads) {
+        float mc = out[2 * W + c], nc = out[c], dc = out[W + c];
+        for (int g = 1; g < kWarps; ++g) add(mc, nc, dc, out[(g * 3 + 2) * W + c], out[g * 3 * W + c], out[(g * 3 + 1) * W + c]);
+        out[c] = nc;
+        out[W + c] = dc;
+    }
+    __syncthreads();
+}
+
 // The history of a slab (W channels of one sequence) is read once, in blocks
-// of kRows rows by W/8 lanes of 8 channels each; exponents are in base 2
-// (k and w scaled by log2 e), and each channel keeps (ref, num, den) with
-// num, den = sums of 2^(y - ref) v and 2^(y - ref) in fp32.
+// of kRows rows, through a ring of blocks in flight that every warp keeps in
+// shared memory.  A lane sums four rows of a block over one group of 32
+// channels, so that the group's parameters and the bias are unpacked once for
+// 32 channels: exponents y = log2(e) (k + w) in base 2, num, den = sums of
+// 2^(y - ref) v and 2^(y - ref) in fp32, and one ref for the channels that
+// share a bias (NH = 1: the group, else each 8), raised when a bound on y
+// (the group's largest value is low + 15 step) passes it by more than 16.
+//
+// A channel that lies so far below its group that its den is below 2^-90 has
+// lost terms to underflow: its share is then summed again with a running
+// maximum per channel.
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
 // other, are cut into equal shares of q blocks, one share a CTA, so ragged
 // lengths balance and a long sequence spreads over many CTAs.  An item that
 // several CTAs share is merged, in CTA order, by the last of them to finish.
-template <typename T, int LPR>
-__global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
+template <typename T, int W, int NH>
+__global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __grid_constant__ Decode p)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
-    constexpr int RPW = 32 / LPR;       // row blocks a warp reads at once
-    constexpr int W = LPR * 8;
+    constexpr int LPR = W / 8;      // lanes of a block
+    constexpr int RPW = 32 / LPR;   // blocks a warp reads at once
+    constexpr int NG = W / 32;      // groups
+    constexpr int kRec = W * 5 / 4, kStageBytes = RPW * kRows * kRec;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int sub = lane / LPR, oct = lane % LPR;
-    __shared__ float part[kWarps][3][W];
-    __shared__ int s_sum[kWarps], s_max[kWarps], s_b, s_first, s_last;
+    const int group = lane % NG, rq = lane % LPR / NG * 4;  // this lane's group, first of its four rows
+    // octets 2, 3 before 0, 1 in the upper four of 8 groups: no bank conflicts
+    const int flip = W == 256 ? group >> 2 : 0;
+    // each warp's blocks in flight; its partial sums [3][W] at the end
+    extern __shared__ __align__(16) uint8_t ring_raw[];
+    auto ring = reinterpret_cast<uint8_t(*)[kStages][kStageBytes]>(ring_raw);
+    auto part = [&](int warp) { return reinterpret_cast<float *>(ring[warp][0]); };
+    static_assert(kStages * kStageBytes >= 8 * 1024, "room for the lanes' sums");
+    const uint32_t mine = smem_u32(ring[warp][0]) + sub * (kRows * kRec) + oct * 16;
+    __shared__ int s_sum[kWarps], s_max[kWarps], s_b, s_first, s_t, s_last;
 
     // this CTA's share [u, u1) of the row blocks
-    int sum = 0, most = 0;
+    int sum = 0, most = 0, t = -1, nb = 0, inc = 0;
     for (int b = tid; b < p.B; b += kThreads) {
-        const int t = p.pos[b], nb = row_blocks(p, t);
+        t = p.pos[b];
+        nb = row_blocks(p, t);
         sum += nb;
         most = max(most, nb);
         if (nb == 0 && b % gridDim.x == blockIdx.x) {  // an inactive sequence
@@ -343,12 +473,22 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
             for (int c = 0; c < p.D; c += 8) store8(static_cast<T *>(p.Z) + b * p.ldz + c, zero);
         }
     }
+    auto scan = [&] {  // inclusive sums of the threads' nb within a warp
+        inc = nb;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += up;
+        }
+    };
+    scan();
     sum = __reduce_add_sync(0xffffffffu, sum);
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
         s_sum[warp] = sum;
         s_max[warp] = most;
     }
+    if (tid == 0) s_b = -1;
     __syncthreads();
     sum = most = 0;
 #pragma unroll
@@ -357,175 +497,296 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
         most = max(most, s_max[k]);
     }
     const int64_t total = (int64_t)sum * p.nslab;
-    const int q = (int)max((total + gridDim.x - 1) / gridDim.x, (int64_t)sqrtf((float)most) + 1);
+    // at least some rounds of the CTA's warps, so that merging a long sequence's
+    // shares does not outweigh summing them
+    const int q = (int)max((total + gridDim.x - 1) / gridDim.x,
+                           (int64_t)min(most, kWarps * ((int)sqrtf((float)most) / 8 + 1)));
     int64_t u = (int64_t)blockIdx.x * q;
     const int64_t u1 = min(total, u + q);
     if (u >= u1) return;
     // the sequence that unit u lies in: blocks before it, over all sequences
     const int target = (int)(u / p.nslab);
-    int before = 0;
-    for (int b0 = 0;; b0 += kThreads) {
-        const int b = b0 + tid;
-        const int nb = b < p.B ? row_blocks(p, p.pos[b]) : 0;
-        int inc = nb;
+    auto locate = [&](int b, int before) {  // before: blocks before this round's
+        int at = before + inc - nb;
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int up = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += up;
-        }
-        __syncthreads();
-        if (lane == 31) s_sum[warp] = inc;
-        if (tid == 0) s_b = -1;
-        __syncthreads();
-        int at = before, all = 0;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
+        for (int k = 0; k < kWarps; ++k)
             if (k < warp) at += s_sum[k];
-            all += s_sum[k];
-        }
-        if (nb && target >= at + inc - nb && target < at + inc) {
+        if (target >= at && target < at + nb) {
             s_b = b;
-            s_first = at + inc - nb;
+            s_first = at;
+            s_t = t;
         }
+    };
+    if (p.B <= kThreads) {
+        locate(tid, 0);
         __syncthreads();
-        before += all;
-        if (s_b >= 0) break;  // total > target: some sequence holds it
+    } else {
+        int before = 0;
+        for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+            t = b0 + tid < p.B ? p.pos[b0 + tid] : -1;
+            nb = row_blocks(p, t);
+            scan();
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = inc;
+            if (tid == 0) s_b = -1;
+            __syncthreads();
+            locate(b0 + tid, before);
+            __syncthreads();
+            if (s_b >= 0) break;  // target < sum: some sequence holds it
+            for (int k = 0; k < kWarps; ++k) before += s_sum[k];
+        }
     }
     int b = s_b;
-    int t = p.pos[b], nb = row_blocks(p, t);
+    if (b < 0) return;
+    t = s_t;
+    nb = row_blocks(p, t);
     int slab = (int)((u - (int64_t)s_first * p.nslab) / nb);
     int blk = (int)((u - (int64_t)s_first * p.nslab) % nb);
 
     for (bool first = true;; first = false) {
         const int n = (int)min((int64_t)(nb - blk), u1 - u);
-        const int ch = slab * W + oct * 8;
         const int32_t *tab = p.table + b * p.ldtab;
-        const T *row = static_cast<const T *>(p.qkv) + b * p.ldq;
-        const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
-        // channels j and j + 4 of the lane's 8 in pairs
-        float2 ref[4], num[4], den[4];
-        float low = -INFINITY;  // the smallest ref, -inf while one is unset
+        const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + slab * W;
+        const float *w[NH];  // bias rows of this lane's octets
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ref[j] = num[j] = den[j] = make_float2(0.f, 0.f);
-        for (int k = warp * RPW + sub; k < n; k += kWarps * RPW) {
-            const int i0 = (blk + k) * kRows;
-            const int page = tab[i0 >> p.shift];
-            const bool ok = page >= 0 && page < p.n_pages;
-            if (!ok && oct == 0) atomicOr(p.status, DC_DEVERR_PAGE);
-            const int rows = ok ? min(kRows, t - i0) : 0;  // rows stored before this call
-            uint8_t *rec = p.pages + record(ok ? page : 0, i0 & (p.page_size - 1), slab, p.nslab, p.page_size, W);
-            uint2 code[kRows], par[kRows];
-            float wl[kRows];
+        for (int h = 0; h < NH; ++h)
+            w[h] = p.w + ((slab * W + group * 32 + (h ^ (2 * flip)) * 8 * (NH > 1)) / p.hs) * p.wh + t * p.ldw + rq;
+        // this warp's blocks: k0, k0 + step, ... < n, RPW neighbours at once
+        constexpr int kStep = kWarps * RPW;
+        const int k0 = warp * RPW + sub;
+        const int rounds = max(0, (n - warp * RPW + kStep - 1) / kStep);
+        uint8_t *pool = p.pages + (size_t)slab * p.page_size * kRec;
+        // pages of a block's halves, -1 behind t and past the share
+        auto pages_of = [&](int it) {
+            const int k = k0 + it * kStep, i0 = (blk + k) * kRows;
+            return make_int2(k < n ? tab[i0 >> p.shift] : -1, k < n && i0 + 8 <= t ? tab[(i0 + 8) >> p.shift] : -1);
+        };
+        auto there = [&](int page) { return (uint32_t)page < (uint32_t)p.n_pages; };
+        auto record_of = [&](int i, int page) {
+            return pool + (size_t)(uint32_t)page * p.page_bytes + (uint32_t)(i & (p.page_size - 1)) * kRec;
+        };
+        // a half without a page is filled with zeros
+        auto fetch = [&](int it, int2 page) {
+            const int i0 = (blk + k0 + it * kStep) * kRows;
+            const uint32_t dst = mine + (it % kStages) * kStageBytes;
+            const bool a = there(page.x), c = there(page.y);
+            const uint8_t *s0 = record_of(i0, a ? page.x : 0) + oct * 16, *s1 = record_of(i0 + 8, c ? page.y : 0) + oct * 16;
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                code[r] = par[r] = make_uint2(0, 0);
-                if (r < rows) {
-                    code[r] = *reinterpret_cast<const uint2 *>(rec + r * (W * 5 / 4) + oct * 8);
-                    par[r] = *reinterpret_cast<const uint2 *>(rec + r * (W * 5 / 4) + W + oct / 4 * 8);
-                }
+            for (int k = 0; k < 5; ++k) cp_async16(dst + k * (LPR * 16), s0 + k * (LPR * 16), a ? 16 : 0);
+#pragma unroll
+            for (int k = 0; k < 5; ++k) cp_async16(dst + (5 + k) * (LPR * 16), s1 + k * (LPR * 16), c ? 16 : 0);
+            cp_async_commit();
+        };
+        // biases of this lane's rows, -inf behind t and without a page
+        auto biases = [&](int it, int2 page, float4 (&x)[NH]) {
+            const int i0 = (blk + k0 + it * kStep) * kRows;
+            const int left = there(rq < 8 ? page.x : page.y) ? t - i0 - rq : -1;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                const float *src = w[h] + i0;
+                if (p.w4 && left >= 3)
+                    x[h] = *reinterpret_cast<const float4 *>(src);
+                else
+                    x[h] = make_float4(left >= 0 ? src[0] : -INFINITY, left >= 1 ? src[1] : -INFINITY,
+                                       left >= 2 ? src[2] : -INFINITY, left >= 3 ? src[3] : -INFINITY);
             }
-            if (rows == kRows && p.w4) {
-                const float4 a = *reinterpret_cast<const float4 *>(w + i0), c = *reinterpret_cast<const float4 *>(w + i0 + 4);
-                wl[0] = a.x; wl[1] = a.y; wl[2] = a.z; wl[3] = a.w;
-                wl[4] = c.x; wl[5] = c.y; wl[6] = c.z; wl[7] = c.w;
-            } else {
+        };
+        // position t: the lanes of its block quantise it, 8 channels each
+        const int tail = nb - 1 - blk - k0;  // rounds * kStep on, if it is this warp's
+        const bool owner = tail >= 0 && tail % kStep == 0 && nb - 1 - blk < n;
+        float fresh[2][8];
+        int home = -1;
+        if (owner) {
+            load8(row + p.D + oct * 8, fresh[0]);
+            load8(row + 2 * p.D + oct * 8, fresh[1]);
+            home = tab[t >> p.shift];
+        }
+        // pages of the blocks in flight, the next one's at hand early
+        int2 page[kStages];
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) wl[r] = r < rows || (ok && i0 + r == t) ? w[i0 + r] : -INFINITY;
-            }
-            if (rows < kRows && ok) {  // position t itself: quantise and append
-                float x[8], st, lo;
-                const uint32_t lanes = 0xfu << (lane & ~3);
-                uint2 c, pr;
-                load8(row + p.D + ch, x);
-                c.x = quantise8(x, st, lo, lanes);
-                pr.x = pack_params(st, lo);
-                load8(row + 2 * p.D + ch, x);
-                c.y = quantise8(x, st, lo, lanes);
-                pr.y = pack_params(st, lo);
-                *reinterpret_cast<uint2 *>(rec + rows * (W * 5 / 4) + oct * 8) = c;
-                if (oct % 4 == 0) *reinterpret_cast<uint2 *>(rec + rows * (W * 5 / 4) + W + oct * 2) = pr;
+        for (int s = 0; s < kStages; ++s) page[s] = pages_of(s);
 #pragma unroll
-                for (int r = 0; r < kRows; ++r)
-                    if (r == rows) {
-                        code[r] = c;
-                        par[r] = pr;
+        for (int s = 0; s < kStages - 1; ++s) fetch(s, page[s]);
+        float4 wn[NH];
+        biases(0, page[0], wn);
+        uint2 nc = make_uint2(0, 0), np = nc;  // its codes and parameters
+        if (owner && there(home)) {
+            float st, lo;
+            const uint32_t lanes = 0xfu << (lane & ~3);
+            nc.x = quantise8(fresh[0], st, lo, lanes);
+            np.x = pack_params(st, lo);
+            nc.y = quantise8(fresh[1], st, lo, lanes);
+            np.y = pack_params(st, lo);
+            uint8_t *rec = record_of(t, home);
+            *reinterpret_cast<uint2 *>(rec + oct * 8) = nc;
+            if (oct % 4 == 0) *reinterpret_cast<uint2 *>(rec + W + oct * 2) = np;
+        }
+
+        // octet o, pair j (factors)
+        f32x2 num[4][4], den[4][4];
+        float ref[NH];
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) num[o][j] = den[o][j] = 0;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) ref[h] = -INFINITY;
+#pragma unroll 1
+        for (int it = 0; it < rounds; ++it) {
+            fetch(it + kStages - 1, page[kStages - 1]);
+            const int2 now = page[0];
+#pragma unroll
+            for (int s = 0; s < kStages - 1; ++s) page[s] = page[s + 1];
+            page[kStages - 1] = pages_of(it + kStages);
+            float4 wl[NH];
+#pragma unroll
+            for (int h = 0; h < NH; ++h) wl[h] = wn[h];
+            biases(it + 1, page[0], wn);
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            uint8_t *stage = ring[warp][it % kStages] + sub * (kRows * kRec);
+            const int at = k0 + it * kStep < n ? t - (blk + k0 + it * kStep) * kRows : -1;
+            if (__any_sync(0xffffffffu, at < kRows || !there(now.x) || !there(now.y))) {
+                // position t itself, or a half without a page
+                if (at >= 0 && oct == 0 && (!there(now.x) || (at >= 8 && !there(now.y)))) atomicOr(p.status, DC_DEVERR_PAGE);
+                if (at >= 0 && at < kRows) {  // and nothing behind it
+                    for (int r = at; r < kRows; ++r) {
+                        *reinterpret_cast<uint2 *>(stage + r * kRec + oct * 8) = r > at ? make_uint2(0, 0) : nc;
+                        if (oct % 4 == 0)
+                            *reinterpret_cast<uint2 *>(stage + r * kRec + W + oct * 2) = r > at ? make_uint2(0, 0) : np;
                     }
+                }
+                __syncwarp();
             }
-            // y = log2(e) (k + w), k = low + step * code
-            float ka[kRows], va[kRows], top = -INFINITY;  // top: a bound on the block's y
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                wl[r] *= kLog2e;
-                ka[r] = base128(par[r].x);
-                va[r] = base128(par[r].y);
-                top = fmax_nan(top, fmaf(fma_bf16(0x430f, par[r].x, ka[r]), kLog2e, wl[r]));
-            }
-            // terms up to 2^16 above a channel's ref are summed as they are;
-            // else the refs rise to the largest exponents so far.  (Exponents
-            // beyond the range of fp32 in base 2, as of a bias of -FLT_MAX,
-            // count as its end.)
-            if (!(low > -1e30f && top <= low + 16.f)) {
+            for (int r = 0; r < 4; ++r) {
+                const uint8_t *rec = stage + (rq + r) * kRec;
+                uint2 code[4];
+                if (kRec % 16 == 0) {
+                    const uint4 c = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 * flip);
+                    const uint4 d = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 - 16 * flip);
+                    code[0] = make_uint2(c.x, c.y);
+                    code[1] = make_uint2(c.z, c.w);
+                    code[2] = make_uint2(d.x, d.y);
+                    code[3] = make_uint2(d.z, d.w);
+                } else {
 #pragma unroll
-                for (int r = 0; r < kRows; ++r)
-                    if (isinf(wl[r]) && ok && (r < rows || i0 + r == t) && !isinf(w[i0 + r]))
-                        wl[r] = copysignf(3.4028234e38f, wl[r]);
-                low = INFINITY;
+                    for (int o = 0; o < 4; ++o)
+                        code[o] = *reinterpret_cast<const uint2 *>(rec + group * 32 + (o ^ (2 * flip)) * 8);
+                }
+                const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + group * 8);
+                // value = low + step c = (low - 16 step) + 32 step (1/2 + c/32),
+                // exact in fp32 unless low outweighs step 2^15 times
+                const float kstep = __uint_as_float(par.x << 16), vstep = __uint_as_float(par.y << 16);
+                const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
+                const float va = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u)), vs = 32.f * vstep;
+                float ks[NH], ka[NH];  // y - ref = ka + ks (1/2 + c/32)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float2 mx, old;
-                    old.x = mx.x = den[j].x == 0.f ? -INFINITY : ref[j].x;
-                    old.y = mx.y = den[j].y == 0.f ? -INFINITY : ref[j].y;
-#pragma unroll
-                    for (int r = 0; r < kRows; ++r) {
-                        const float2 y = __ffma2_rn(value2(code[r].x, j, par[r].x, ka[r]),
-                                                    make_float2(kLog2e, kLog2e), make_float2(wl[r], wl[r]));
-                        mx.x = fmax_nan(mx.x, y.x);
-                        mx.y = fmax_nan(mx.y, y.y);
+                for (int h = 0; h < NH; ++h) {
+                    const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
+                    ks[h] = kstep * (32.f * kLog2e);
+                    ka[h] = fmaf(klow, kLog2e, x * kLog2e);
+                    if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
+                        // a finite bias of such size (a mask of -FLT_MAX)
+                        // absorbs the keys, in fp32 as in 64 bits
+                        ks[h] = 0.f;
+                        ka[h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
                     }
-                    low = fminf(low, fminf(mx.x, mx.y));
-                    auto raise = [](float mx, float old, float &ref, float &num, float &den) {
-                        if (mx == -INFINITY) return;
-                        const float scale = ex2(old - mx);
-                        num *= scale;
-                        den *= scale;
-                        ref = mx;
-                    };
-                    raise(mx.x, old.x, ref[j].x, num[j].x, den[j].x);
-                    raise(mx.y, old.y, ref[j].y, num[j].y, den[j].y);
+                    const float top = fmaf(ks[h], 31.f / 32.f, ka[h]);
+                    if (!(top <= ref[h] + 16.f)) {  // also where either is NaN
+                        const float scale = ex2(ref[h] - top);
+#pragma unroll
+                        for (int o = 0; o < 4; ++o)
+                            if (NH == 1 || o == h)
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    num[o][j] = mul2(num[o][j], pack2(scale, scale));
+                                    den[o][j] = mul2(den[o][j], pack2(scale, scale));
+                                }
+                        ref[h] = top;
+                    }
+                    if (ref[h] != -INFINITY) ka[h] -= ref[h];
+                }
+                f32x2 ks2[NH], ka2[NH];
+                const f32x2 vs2 = pack2(vs, vs), va2 = pack2(va, va);
+#pragma unroll
+                for (int h = 0; h < NH; ++h) {
+                    ks2[h] = pack2(ks[h], ks[h]);
+                    ka2[h] = pack2(ka[h], ka[h]);
+                }
+#pragma unroll
+                for (int o = 0; o < 4; ++o) {
+                    const int h = NH == 1 ? 0 : o;
+                    const uint32_t k0 = code[o].x << 3 & 0x78787878u, k1 = code[o].x >> 1 & 0x78787878u;
+                    const uint32_t v0 = code[o].y << 3 & 0x78787878u, v1 = code[o].y >> 1 & 0x78787878u;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 y = unpack2(fma2(factors(k0, k1, j), ks2[h], ka2[h]));
+                        const f32x2 e = pack2(ex2(y.x), ex2(y.y));
+                        const f32x2 v = fma2(factors(v0, v1, j), vs2, va2);
+                        num[o][j] = fma2(e, v, num[o][j]);
+                        den[o][j] = add2(den[o][j], e);
+                    }
                 }
             }
-#pragma unroll
-            for (int r = 0; r < kRows; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float2 y = __ffma2_rn(value2(code[r].x, j, par[r].x, ka[r]), make_float2(kLog2e, kLog2e),
-                                          make_float2(wl[r], wl[r]));
-                    y = __fadd2_rn(y, make_float2(-ref[j].x, -ref[j].y));
-                    const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                    num[j] = __ffma2_rn(e, value2(code[r].y, j, par[r].y, va[r]), num[j]);
-                    den[j] = __fadd2_rn(den[j], e);
-                }
+            __syncwarp();  // the stage may be filled again
         }
-        // blocks of a warp, then warps
-        float fr[8], fu[8], fe[8];
+        cp_async_wait<0>();
+        __syncwarp();
+        // the lanes of a group: one ref, then sums over their NL lanes
+        constexpr int NL = 32 / NG;
+        float *sums = part(warp);  // [NL][2][W], then ref, num, den [3][W]
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            fe[j] = j < 4 ? den[j & 3].x : den[j & 3].y;
-            fu[j] = j < 4 ? num[j & 3].x : num[j & 3].y;
-            fr[j] = fe[j] == 0.f ? -INFINITY : j < 4 ? ref[j & 3].x : ref[j & 3].y;
+        for (int h = 0; h < NH; ++h) {
+            float r = ref[h];
 #pragma unroll
-            for (int o = LPR; o < 32; o *= 2) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, fr[j], o);
-                const float n2 = __shfl_xor_sync(0xffffffffu, fu[j], o);
-                const float d2 = __shfl_xor_sync(0xffffffffu, fe[j], o);
-                join(fr[j], fu[j], fe[j], m2, n2, d2);
+            for (int x = NG; x < 32; x *= 2) r = fmax_nan(r, __shfl_xor_sync(0xffffffffu, r, x));
+            const float scale = ref[h] == -INFINITY ? 0.f : ex2(ref[h] - r);
+            ref[h] = r;
+#pragma unroll
+            for (int o = 0; o < 4; ++o)
+                if (NH == 1 || o == h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        num[o][j] = mul2(num[o][j], pack2(scale, scale));
+                        den[o][j] = mul2(den[o][j], pack2(scale, scale));
+                    }
+        }
+#pragma unroll
+        for (int o = 0; o < 4; ++o) {
+            float *to = sums + (lane / NG) * 2 * W + group * 32 + (o ^ (2 * flip)) * 8;
+            float2 m[4], d[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[j] = unpack2(num[o][j]);
+                d[j] = unpack2(den[o][j]);
+            }
+            store8(to, {m[0].x, m[2].x, m[0].y, m[2].y, m[1].x, m[3].x, m[1].y, m[3].y});
+            store8(to + W, {d[0].x, d[2].x, d[0].y, d[2].y, d[1].x, d[3].x, d[1].y, d[3].y});
+        }
+        __syncwarp();
+        float sn[W / 32], sd[W / 32];
+#pragma unroll
+        for (int k = 0; k < W / 32; ++k) {
+            sn[k] = sd[k] = 0.f;
+#pragma unroll (NL < 8 ? NL : 8)
+            for (int l = 0; l < NL; ++l) {
+                sn[k] += sums[l * 2 * W + k * 32 + lane];
+                sd[k] += sums[(l * 2 + 1) * W + k * 32 + lane];
             }
         }
-        if (sub == 0) {
-            store8(&part[warp][0][oct * 8], fr);
-            store8(&part[warp][1][oct * 8], fu);
-            store8(&part[warp][2][oct * 8], fe);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < W / 32; ++k) {
+            sums[W + k * 32 + lane] = sn[k];
+            sums[2 * W + k * 32 + lane] = sd[k];
         }
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            if (lane / NG == o) {
+                const float r = ref[o % NH];
+                store8(sums + group * 32 + (o ^ (2 * flip)) * 8, {r, r, r, r, r, r, r, r});
+            }
         __syncthreads();
         constexpr int CPT = (W + kThreads - 1) / kThreads;  // channels a thread finishes
         float fm[CPT], fn[CPT], fd[CPT];
@@ -533,11 +794,11 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
         for (int k = 0; k < CPT; ++k) {
             const int c = tid + k * kThreads;
             if (c >= W) continue;
-            fm[k] = part[0][0][c];
-            fn[k] = part[0][1][c];
-            fd[k] = part[0][2][c];
+            fm[k] = part(0)[c];
+            fn[k] = part(0)[W + c];
+            fd[k] = part(0)[2 * W + c];
 #pragma unroll
-            for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part[g][0][c], part[g][1][c], part[g][2][c]);
+            for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part(g)[c], part(g)[W + c], part(g)[2 * W + c]);
         }
         bool finish = n == nb;
         if (!finish) {  // shared with other CTAs
@@ -569,20 +830,44 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
                     if (c >= W) continue;
                     fm[k] = -INFINITY;
                     fn[k] = fd[k] = 0.f;
-                    for (int g = j0; g <= j1; ++g) {
-                        // the item is CTA g's first unless it begins inside g's share
-                        const float *src = p.part + ((int64_t)g * 2 + (u_item > (int64_t)g * q)) * 3 * W + c;
-                        join(fm[k], fn[k], fd[k], __ldcg(src), __ldcg(src + W), __ldcg(src + 2 * W));
+                    for (int g0 = j0; g0 <= j1; g0 += 4) {
+                        float x[4][3];
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            // the item is CTA g's first unless it begins inside g's share
+                            const int g = min(g0 + d, j1);
+                            const float *src = p.part + ((int64_t)g * 2 + (u_item > (int64_t)g * q)) * 3 * W + c;
+                            x[d][0] = __ldcg(src);
+                            x[d][1] = __ldcg(src + W);
+                            x[d][2] = __ldcg(src + 2 * W);
+                        }
+#pragma unroll
+                        for (int d = 0; d < 4; ++d)
+                            if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][0], x[d][1], x[d][2]);
                     }
                 }
             }
         }
         if (finish) {
+            int lost = 0;
+#pragma unroll
+            for (int k = 0; k < CPT; ++k)
+                if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-90f) lost = 1;
+            if (__syncthreads_or(lost)) {
+                resum<W>(p, b, slab, t, part(0));
+#pragma unroll
+                for (int k = 0; k < CPT; ++k) {
+                    const int c = tid + k * kThreads;
+                    if (c >= W) continue;
+                    fn[k] = part(0)[c];
+                    fd[k] = part(0)[W + c];
+                }
+            }
 #pragma unroll
             for (int k = 0; k < CPT; ++k) {
                 const int c = tid + k * kThreads;
                 if (c >= W) continue;
-                const float qv = to_f<T>(row[slab * W + c]);
+                const float qv = to_f<T>(row[c]);
                 static_cast<T *>(p.Z)[b * p.ldz + slab * W + c] =
                     from_f<T>(fd[k] == 0.f ? 0.f : sigm(qv) * (fn[k] / fd[k]));
             }
@@ -592,8 +877,10 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
         blk = 0;
         if (++slab == p.nslab) {
             slab = 0;
-            do t = p.pos[++b];  // u < total: there is another active one
-            while ((nb = row_blocks(p, t)) == 0);
+            do {  // u < total: there is another active one
+                if (++b >= p.B) return;
+                t = p.pos[b];
+            } while ((nb = row_blocks(p, t)) == 0);
         }
         __syncthreads();  // part is reused
     }
@@ -601,15 +888,35 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(Decode p)
 
 static int decode_grid() { return kResident * sm_count(); }
 
+template <typename T, int W>
+static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
+{
+    const dim3 grid((unsigned)decode_grid()), block(kThreads);
+    constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
+    auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
+    // once per device (the attribute belongs to the device's context)
+    static std::atomic<uint64_t> ready[2];
+    std::atomic<uint64_t> &done = ready[p.hs % 32 == 0];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
+    return launch_pdl(kernel, grid, block, smem, st, 1, p);
+}
+
 template <typename T>
 static cudaError_t launch_decode(const Decode &p, cudaStream_t st)
 {
-    const dim3 grid((unsigned)decode_grid()), block(kThreads);
     switch (p.W) {
-        case 256: return launch_pdl(decode_kernel<T, 32>, grid, block, 0, st, 1, p);
-        case 128: return launch_pdl(decode_kernel<T, 16>, grid, block, 0, st, 1, p);
-        case 64: return launch_pdl(decode_kernel<T, 8>, grid, block, 0, st, 1, p);
-        default: return launch_pdl(decode_kernel<T, 4>, grid, block, 0, st, 1, p);
+        case 256: return launch_slab<T, 256>(p, st);
+        case 128: return launch_slab<T, 128>(p, st);
+        case 64: return launch_slab<T, 64>(p, st);
+        default: return launch_slab<T, 32>(p, st);
     }
 }
 
@@ -730,6 +1037,7 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     p.page_size = page_size;
     p.cap = (int)std::min<int64_t>(Tmax, (int64_t)ldtab * page_size);
     for (p.shift = 3; 1 << p.shift < page_size;) ++p.shift;
+    p.page_bytes = (uint32_t)(page_size * (int64_t)D * 5 / 4);
     p.w4 = aligned16(w) && ldw % 4 == 0 && head_stride_w % 4 == 0;
     p.counter = static_cast<int *>(workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) +
