@@ -104,79 +104,6 @@ __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One group's quantisation by the 4 lanes (xor 1, 2) that hold its 32 values:
-// step and low (bf16 values, the same on the 4 lanes), this lane's 8 codes.
-// `lanes`: the lanes that take part, whole groups.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float &step, float &low,
-                                              uint32_t lanes = 0xffffffffu)
-{
-    float mn = x[0], mx = x[0];
-    int bad = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        mn = fminf(mn, x[j]);
-        mx = fmaxf(mx, x[j]);
-        bad |= !(fabsf(x[j]) <= kBig);
-    }
-#pragma unroll
-    for (int o = 1; o <= 2; o *= 2) {
-        mn = fminf(mn, __shfl_xor_sync(lanes, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(lanes, mx, o));
-        bad |= __shfl_xor_sync(lanes, bad, o);
-    }
-    if (bad) {
-        step = __uint_as_float(0x7fff0000u);
-        low = 0.f;
-        return 0;
-    }
-    uint32_t cut = __float_as_uint(mn) & 0xffff0000u;  // towards zero
-    if (__uint_as_float(cut) > mn) cut += 0x10000u;
-    low = __uint_as_float(cut == 0x80000000u ? 0u : cut);  // -0 is stored as 0
-    const float up = __fdiv_ru(__fsub_ru(mx, low), 15.f);
-    step = __uint_as_float((__float_as_uint(up) + 0xffffu) & 0xffff0000u);
-    if (step == 0.f) {  // -0 - 0 among them
-        step = 0.f;
-        return 0;
-    }
-    // (x - low) / step, rounded: off by at most 2^-22 of its value (tiny steps
-    // are scaled first), so the nearest whole number is the code unless that
-    // lies 0.5 away to within 1e-5; there the borders decide
-    const float scale = step < 1e-30f ? 0x1p100f : 1.f, inv = __frcp_rn(step * scale);
-    float c[8], worst = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float q = (x[j] - low) * scale * inv;
-        c[j] = (q + 12582912.f) - 12582912.f;
-        worst = fmaxf(worst, fabsf(q - c[j]));
-    }
-    if (worst > 0.49999f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (x[j] < __fmaf_ru(step, c[j] - 0.5f, low))
-                c[j] -= 1.f;
-            else if (x[j] >= __fmaf_ru(step, c[j] + 0.5f, low))
-                c[j] += 1.f;
-        }
-    }
-    // four codes are the digits of a number below 2^16
-    const float lo4 = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
-    const float hi4 = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
-    return __byte_perm(__float_as_uint(lo4), __float_as_uint(hi4), 0x5410);
-}
-
-__device__ __forceinline__ uint32_t pack_params(float step, float low)
-{
-    return (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
-}
-
-// The 8 values that codes stand for.
-__device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (&x)[8])
-{
-    const float step = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
-}
-
 // Pairs of fp32 numbers in a 64-bit register (the type that keeps a pair of
 // equal numbers in place: float2 operands were copied at every use).
 typedef unsigned long long f32x2;
@@ -210,6 +137,116 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// a * b + c rounded up
+__device__ __forceinline__ f32x2 fma2_ru(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rp.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Largest / smallest of three (NaN if one is, respectively ignoring NaN).
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c)
+{
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// One group's quantisation by the 4 lanes (xor 1, 2) that hold its 32 values:
+// step and low (bf16 values, the same on the 4 lanes), this lane's 8 codes,
+// as numbers in c and packed.  `lanes`: the lanes that take part, whole
+// groups.  x is scratch.
+__device__ __forceinline__ uint32_t quantise8(float (&x)[8], float &step, float &low, float (&c)[8],
+                                              uint32_t lanes = 0xffffffffu)
+{
+    float mx = max3_nan(max3_nan(x[0], x[1], x[2]), max3_nan(x[3], x[4], x[5]), max3_nan(x[6], x[7], x[7]));
+    float mn = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), min3(x[6], x[7], x[7]));
+#pragma unroll
+    for (int o = 1; o <= 2; o *= 2) {
+        const float other = __shfl_xor_sync(lanes, mx, o);
+        mx = max3_nan(mx, other, other);
+        mn = fminf(mn, __shfl_xor_sync(lanes, mn, o));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = 0.f;
+    if (!(mx <= kBig && mn >= -kBig)) {
+        step = __uint_as_float(0x7fff0000u);
+        low = 0.f;
+        return 0;
+    }
+    uint32_t cut = __float_as_uint(mn) & 0xffff0000u;  // towards zero
+    if (__uint_as_float(cut) > mn) cut += 0x10000u;
+    low = __uint_as_float(cut == 0x80000000u ? 0u : cut);  // -0 is stored as 0
+    // the smallest bf16 whose 15-fold (exact in fp32) is not below mx - low
+    // (then not below that rounded up): the estimate is at most one off
+    const float range = fabsf(__fsub_ru(mx, low));
+    uint32_t s = (__float_as_uint(range * (1.f / 15.f)) + 0xffffu) & 0xffff0000u;
+    if (15.f * __uint_as_float(s) < range)
+        s += 0x10000u;
+    else if (s && 15.f * __uint_as_float(s - 0x10000u) >= range)
+        s -= 0x10000u;
+    step = __uint_as_float(s);
+    if (step == 0.f) return 0;
+    float st = step, lo = low;
+    if (step < 1e-30f) {  // then every value is small enough to scale, exactly
+        st *= 0x1p100f;
+        lo *= 0x1p100f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= 0x1p100f;
+    }
+    // (x - low) / step is off by at most 2^-21 of its value, so the nearest
+    // whole number is the code unless that lies 0.5 away to within 1e-5 (as
+    // often with bf16 values); then the border between the two decides
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(st));
+    const f32x2 inv2 = pack2(inv, inv), lo2 = pack2(lo, lo);
+    float2 r[4];
+    float worst = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x2 d = add2(pack2(x[2 * j], x[2 * j + 1]), lo2 ^ 0x8000000080000000ull);
+        const f32x2 k = add2(fma2(d, inv2, pack2(12582912.f, 12582912.f)), pack2(-12582912.f, -12582912.f));
+        r[j] = unpack2(fma2(d, inv2, k ^ 0x8000000080000000ull));
+        worst = fmaxf(worst, fmaxf(fabsf(r[j].x), fabsf(r[j].y)));
+        c[2 * j] = unpack2(k).x;
+        c[2 * j + 1] = unpack2(k).y;
+    }
+    if (worst > 0.49999f) {
+        const f32x2 st2 = pack2(st, st);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x2 border = add2(pack2(c[2 * j], c[2 * j + 1]), pack2(copysignf(0.5f, r[j].x), copysignf(0.5f, r[j].y)));
+            const float2 y = unpack2(fma2_ru(st2, border, lo2));
+            const float2 k = unpack2(add2(border, pack2(x[2 * j] >= y.x ? 0.5f : -0.5f, x[2 * j + 1] >= y.y ? 0.5f : -0.5f)));
+            c[2 * j] = k.x;
+            c[2 * j + 1] = k.y;
+        }
+    }
+    // four codes are the digits of a number below 2^16
+    const float lo4 = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f;
+    const float hi4 = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + 8388608.f;
+    return __byte_perm(__float_as_uint(lo4), __float_as_uint(hi4), 0x5410);
+}
+
+__device__ __forceinline__ uint32_t pack_params(float step, float low)
+{
+    return (__float_as_uint(step) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+}
+
+// The 8 values that codes stand for.
+__device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (&x)[8])
+{
+    const float step = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
+}
 
 // Two codes as fp32 numbers 1/2 + c/32: the codes of a word are masked into
 // bits 3..6 of its bytes (8 codes: two words, of even and odd channels), and
@@ -233,32 +270,35 @@ struct Write {
     const void *k, *v;
     int64_t ld;
     const int32_t *slots;
-    int n, D, W, page_size, n_pages;
+    int n, D, W, page_size, n_pages, shift;  // page_size = 1 << shift
+    uint32_t page_bytes;
     uint8_t *pages;
     void *vk, *vv;
     int64_t ldv;
     int *status;
 };
 
-// One lane per 8 channels of a row (k and v); rows with a negative slot are
-// left out.
+constexpr int kWriteWarps = 8;
+
+// A lane per 8 channels of a row (k and v), `span` lanes a row: a warp takes
+// 256 channels of a row (blockIdx.y which of them), or 32/span rows of fewer.
+// Rows with a negative slot are left out.  HBM-bound.
 template <typename T>
-__global__ void __launch_bounds__(256) write_kernel(Write p)
+__global__ void __launch_bounds__(32 * kWriteWarps) write_kernel(const __grid_constant__ Write p, int span)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
-    const int octs = p.D / 8;
-    const int64_t total = (int64_t)p.n * octs;  // a multiple of 4: groups stay within a warp
-    const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-    const int64_t first = (int64_t)blockIdx.x * blockDim.x + (threadIdx.x & ~31);
-    for (int64_t base = first; base < total; base += stride) {
-        const int64_t at = base + (threadIdx.x & 31);
-        const bool in = at < total;
-        const int row = in ? (int)(at / octs) : 0;
-        const int ch = in ? (int)(at % octs) * 8 : 0;
-        const int slot = in ? p.slots[row] : -1;
+    const int lane = threadIdx.x & 31, rows = 32 / span;
+    const int ch = blockIdx.y * 256 + lane % span * 8;
+    const int at = ch & (p.W - 1), rec_bytes = p.W / 4 * 5;
+    uint8_t *base = p.pages + (size_t)(ch / p.W) * p.page_size * rec_bytes;
+    const int step = gridDim.x * kWriteWarps * rows;
+    // the warp's rows are the same number of rounds away for all its lanes
+    for (int first = (blockIdx.x * kWriteWarps + (threadIdx.x >> 5)) * rows; first < p.n; first += step) {
+        const int row = first + lane / span;
+        const int slot = row < p.n && ch < p.D ? p.slots[row] : -1;
         const bool ok = slot >= 0 && slot < (int64_t)p.n_pages * p.page_size;
-        float k[8] = {}, v[8] = {};
+        float k[8] = {}, v[8] = {}, kc[8], vc[8];
         if (ok) {
             load8(static_cast<const T *>(p.k) + row * p.ld + ch, k);
             load8(static_cast<const T *>(p.v) + row * p.ld + ch, v);
@@ -266,17 +306,19 @@ __global__ void __launch_bounds__(256) write_kernel(Write p)
             atomicOr(p.status, DC_DEVERR_PAGE);
         }
         float ks, kl, vs, vl;
-        const uint32_t kc = quantise8(k, ks, kl), vc = quantise8(v, vs, vl);
+        const uint32_t kb = quantise8(k, ks, kl, kc), vb = quantise8(v, vs, vl, vc);
+        if (step > INT32_MAX - first) first = INT32_MAX - step;  // the last round
         if (!ok) continue;
-        const uint32_t kp = pack_params(ks, kl), vp = pack_params(vs, vl);
-        uint8_t *rec = p.pages + record(slot / p.page_size, slot % p.page_size, ch / p.W, p.D / p.W,
-                                        p.page_size, p.W);
-        const int c = ch % p.W;
-        *reinterpret_cast<uint2 *>(rec + c) = make_uint2(kc, vc);
-        if (c % 32 == 0) *reinterpret_cast<uint2 *>(rec + p.W + c / 4) = make_uint2(kp, vp);
+        uint8_t *rec = base + (size_t)(slot >> p.shift) * p.page_bytes + (slot & (p.page_size - 1)) * rec_bytes;
+        *reinterpret_cast<uint2 *>(rec + at) = make_uint2(kb, vb);
+        if (at % 32 == 0)
+            *reinterpret_cast<uint2 *>(rec + p.W + at / 4) = make_uint2(pack_params(ks, kl), pack_params(vs, vl));
         if (p.vk) {
-            values8(kc, kp, k);
-            values8(vc, vp, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                k[j] = fmaf(ks, kc[j], kl);
+                v[j] = fmaf(vs, vc[j], vl);
+            }
             store8(static_cast<T *>(p.vk) + row * p.ldv + ch, k);
             store8(static_cast<T *>(p.vv) + row * p.ldv + ch, v);
         }
@@ -611,11 +653,11 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         biases(0, page[0], wn);
         uint2 nc = make_uint2(0, 0), np = nc;  // its codes and parameters
         if (owner && there(home)) {
-            float st, lo;
+            float st, lo, c[8];
             const uint32_t lanes = 0xfu << (lane & ~3);
-            nc.x = quantise8(fresh[0], st, lo, lanes);
+            nc.x = quantise8(fresh[0], st, lo, c, lanes);
             np.x = pack_params(st, lo);
-            nc.y = quantise8(fresh[1], st, lo, lanes);
+            nc.y = quantise8(fresh[1], st, lo, c, lanes);
             np.y = pack_params(st, lo);
             uint8_t *rec = record_of(t, home);
             *reinterpret_cast<uint2 *>(rec + oct * 8) = nc;
@@ -922,7 +964,8 @@ static cudaError_t launch_decode(const Decode &p, cudaStream_t st)
 
 static int check_pool(int D, int n_pages, int page_size)
 {
-    if (D <= 0 || D % 32) return fail(DC_ERR_INVALID, "D must be a positive multiple of 32 (got %d)", D);
+    if (D <= 0 || D % 32 || D > 1 << 20)
+        return fail(DC_ERR_INVALID, "D must be a positive multiple of 32, at most 2^20 (got %d)", D);
     if (n_pages <= 0) return fail(DC_ERR_INVALID, "n_pages must be positive");
     if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
         return fail(DC_ERR_INVALID, "page_size must be 8, 16, 32, 64, 128 or 256 (got %d)", page_size);
@@ -955,7 +998,7 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
     clear_error();
     DC_TRY(check_pool(D, n_pages, page_size));
     if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
-    if (n < 0) return fail(DC_ERR_INVALID, "bad row count %d", n);
+    if (n < 0 || n > INT32_MAX - 64) return fail(DC_ERR_INVALID, "bad row count %d", n);
     if (n == 0) return DC_OK;
     if (!k || !v || !slots || !pages) return fail(DC_ERR_INVALID, "null pointer");
     if (!values_k != !values_v) return fail(DC_ERR_INVALID, "values_k and values_v go together");
@@ -973,6 +1016,8 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
     p.D = D;
     p.W = slab_width(D);
     p.page_size = page_size;
+    for (p.shift = 3; 1 << p.shift < page_size;) ++p.shift;
+    p.page_bytes = (uint32_t)(page_size * (int64_t)D * 5 / 4);
     p.n_pages = n_pages;
     p.pages = static_cast<uint8_t *>(pages);
     p.vk = values_k;
@@ -982,10 +1027,12 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("kv4_write", st);
-    const int64_t blocks = ((int64_t)n * (D / 8) + 255) / 256;
-    const dim3 grid((unsigned)std::min<int64_t>(blocks, (int64_t)sm_count() * 64));
-    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(write_kernel<float>, grid, dim3(256), 0, st, 1, p)
-                                : launch_pdl(write_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, 1, p));
+    int span = 4;  // lanes a row
+    while (span < 32 && span * 8 < D) span *= 2;
+    const int chunks = (D + 255) / 256, rows = kWriteWarps * (32 / span);
+    const dim3 grid(std::min((n - 1) / rows + 1, std::max(1, sm_count() * 32 / chunks)), chunks), block(32 * kWriteWarps);
+    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(write_kernel<float>, grid, block, 0, st, 1, p, span)
+                                : launch_pdl(write_kernel<__nv_bfloat16>, grid, block, 0, st, 1, p, span));
     return DC_OK;
 }
 

@@ -344,7 +344,7 @@ int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_s
                    int ld_slots, int32_t *row_start, void *stream);
 
 /* Paged 4-bit history of one layer: n_pages pages of page_size positions of D
- * channels (a multiple of 32), dc_kv4_pages_size bytes, 16-byte aligned:
+ * channels (a multiple of 32, at most 2^20), dc_kv4_pages_size bytes, 16-byte aligned:
  * [n_pages][D/W][page_size][5W/4], W the largest of 256, 128, 64, 32 that
  * divides D.  A record holds, per 8 channels, 4 bytes of k codes and 4 of v
  * codes (channel j in bits 4j..4j+3), then per group of 32 channels four
