@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/dart_cuda_b200.h"
@@ -58,6 +59,23 @@ struct KernelTimer {
 bool profiling_enabled();
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Raises a kernel's limit of dynamic shared memory once per device.
+struct SmemOnce {
+    std::atomic<uint64_t> done{0};
+    template <typename K>
+    cudaError_t set(K *kernel, int bytes)
+    {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+        if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 // Launch with programmatic stream serialisation (the kernel calls
 // grid_dep_wait() before its first dependent memory access) and, when

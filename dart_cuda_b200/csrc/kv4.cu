@@ -30,7 +30,6 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "dc_internal.h"
 #include "dc_ptx.cuh"
@@ -936,18 +935,9 @@ static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
     const dim3 grid((unsigned)decode_grid()), block(kThreads);
     constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
     auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
-    // once per device (the attribute belongs to the device's context)
-    static std::atomic<uint64_t> ready[2];
-    std::atomic<uint64_t> &done = ready[p.hs % 32 == 0];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    static SmemOnce once[2];
+    const cudaError_t e = once[p.hs % 32 == 0].set(kernel, smem);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-        done.fetch_or(bit, std::memory_order_relaxed);
-    }
     return launch_pdl(kernel, grid, block, smem, st, 1, p);
 }
 

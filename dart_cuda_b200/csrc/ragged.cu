@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "dc_internal.h"
 #include "dc_ptx.cuh"
@@ -43,6 +44,7 @@ struct Tables {
     int ldtab;
     int32_t *slots;
     int n_slots, ld_slots;
+    int slots4;  // slots is 16-byte aligned
     int32_t *row_start;
     int *status;
 };
@@ -89,20 +91,24 @@ __device__ __forceinline__ void scan2(int64_t &a, int &b, int64_t &ta, int &tb)
     b = ib - b + (warp ? before_b : 0);
 }
 
-__global__ void __launch_bounds__(kTabThreads) tables_kernel(Tables p)
+// Every CTA finds the prefix sums (rounds of kTabThreads requests) and writes
+// its part of the table entries and slots, up to four slots a thread.  Latency-bound:
+// the chain is lengths, two prefix sums, free pages, stores.
+__global__ void __launch_bounds__(kTabThreads) tables_kernel(const __grid_constant__ Tables p)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
     // requests of this round: first token, tokens, pages there and needed,
     // free page of table column 0 (column c >= have takes free[base + c]),
-    // packed row
+    // packed row (none counts behind the slots)
     __shared__ int s_start[kTabThreads], s_count[kTabThreads], s_have[kTabThreads], s_last[kTabThreads],
-        s_base[kTabThreads];
-    __shared__ int64_t s_row[kTabThreads + 1];
+        s_base[kTabThreads], s_row[kTabThreads + 1];
     const int ps = 1 << p.shift, tid = threadIdx.x;
+    const int64_t thread = (int64_t)blockIdx.x * kTabThreads + tid, threads = (int64_t)gridDim.x * kTabThreads;
     const int head = min(max(0, *p.head), p.n_free);
     int64_t rows = 0;
     int pages = 0, err = 0;
+    auto clip = [&](int64_t x) { return (int)min(x, (int64_t)INT32_MAX); };
     for (int b0 = 0; b0 < p.B; b0 += kTabThreads) {
         const int b = b0 + tid, nb = min(kTabThreads, p.B - b0);
         int start = 0, count = 0, have = 0, last = 0;
@@ -123,53 +129,85 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(Tables p)
         s_count[tid] = count;
         s_have[tid] = have;
         s_last[tid] = last;
-        s_row[tid] = rows + row;
+        s_row[tid] = clip(rows + row);
         s_base[tid] = (int)min((int64_t)INT32_MAX / 2, (int64_t)head + pages + first) - have;
-        if (tid == 0) s_row[nb] = rows + trow;
-        if (b < p.B && p.row_start) p.row_start[b] = (int)min(rows + row, (int64_t)INT32_MAX);
+        if (tid == 0) s_row[nb] = clip(rows + trow);
+        if (b < p.B && p.row_start && blockIdx.x == 0) p.row_start[b] = clip(rows + row);
         if (need && (int64_t)head + pages + first + need > p.n_free) err = 1;
         __syncthreads();
         // table entries: a warp per request
-        for (int r = tid >> 5; r < nb; r += kTabThreads / 32) {
+        for (int r = (int)(thread >> 5); r < nb; r += (int)(threads >> 5)) {
             for (int c = s_have[r] + (tid & 31); c < s_last[r]; c += 32) {
                 const int at = s_base[r] + c;
                 p.table[(int64_t)(b0 + r) * p.ldtab + c] = at < p.n_free ? p.free_pages[at] : -1;
             }
         }
-        // slots: token j of request r
-        auto slot_of = [&](int r, int j) {
-            const int64_t t = (int64_t)s_start[r] + j;
-            const int64_t c = t >> p.shift;
-            if (c >= p.ldtab) return -1;
-            const int at = s_base[r] + (int)c;
-            int page = -1;
-            if (c < s_have[r])  // the page that start ends in
-                page = p.table[(int64_t)(b0 + r) * p.ldtab + c];
-            else if (at < p.n_free)
-                page = p.free_pages[at];
-            const int64_t slot = (int64_t)page * ps + (t & (ps - 1));
-            if (page < 0 || slot > INT32_MAX) {
-                err = 1;
-                return -1;
+        // slots i0 .. i0+per-1 of [from, to); where(i, r, j): the request of
+        // slot i and which of its tokens, or false
+        auto write = [&](int64_t i0, int per, int64_t from, int64_t to, auto where) {
+            int v[4], at_r = -1, at_c = -1, page = -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = -1;
+                const int64_t i = i0 + k;
+                int r, j;
+                if (k >= per || i < from || i >= to || !where(i, r, j)) continue;
+                const int64_t t = (int64_t)s_start[r] + j;
+                if (t >> p.shift >= p.ldtab) continue;
+                const int c = (int)(t >> p.shift);
+                if (r != at_r || c != at_c) {  // another page than the last slot's
+                    at_r = r;
+                    at_c = c;
+                    page = -1;
+                    if (c < s_have[r])  // the page that start ends in
+                        page = p.table[(int64_t)(b0 + r) * p.ldtab + c];
+                    else if (s_base[r] + c < p.n_free)
+                        page = p.free_pages[s_base[r] + c];
+                }
+                const int64_t slot = (int64_t)page * ps + (t & (ps - 1));
+                if (page < 0 || slot > INT32_MAX)
+                    err = 1;
+                else
+                    v[k] = (int)slot;
             }
-            return (int)slot;
+            if (per == 4 && p.slots4 && i0 >= from && i0 + 4 <= to) {
+                *reinterpret_cast<int4 *>(p.slots + i0) = make_int4(v[0], v[1], v[2], v[3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (k < per && i0 + k >= from && i0 + k < to) p.slots[i0 + k] = v[k];
+            }
         };
+        // few slots: one a thread, so that their pages are read side by side
+        auto per_thread = [&](int64_t n) { return n <= threads ? 1 : 4; };
         if (p.slots && p.ld_slots) {
-            const int64_t i0 = (int64_t)b0 * p.ld_slots, i1 = (int64_t)(b0 + nb) * p.ld_slots;
-            for (int64_t i = i0 + tid; i < i1; i += kTabThreads) {
-                const int r = (int)((i - i0) / p.ld_slots), j = (int)((i - i0) % p.ld_slots);
-                p.slots[i] = j < s_count[r] ? slot_of(r, j) : -1;
-            }
+            const int64_t from = (int64_t)b0 * p.ld_slots, to = (int64_t)(b0 + nb) * p.ld_slots;
+            const int per = per_thread(to - from);
+            for (int64_t i = (from & -per) + per * thread; i < to; i += per * threads)
+                write(i, per, from, to, [&](int64_t i, int &r, int &j) {
+                    const uint32_t d = (uint32_t)(i - from);  // below n_slots
+                    r = (int)(d / (uint32_t)p.ld_slots);
+                    j = (int)(d - (uint32_t)r * (uint32_t)p.ld_slots);
+                    return j < s_count[r];
+                });
             if (b < p.B && count > p.ld_slots) err = 1;
         } else if (p.slots) {
-            for (int64_t i = s_row[0] + tid; i < min(s_row[nb], (int64_t)p.n_slots); i += kTabThreads) {
-                int lo = 0, hi = nb - 1;  // last request that starts at or before i
+            const int64_t from = s_row[0], to = min(s_row[nb], p.n_slots);
+            const int per = per_thread(to - from);
+            for (int64_t i = (from & -per) + per * thread; i < to; i += per * threads) {
+                int lo = 0, hi = nb - 1;  // last request that starts at or before the first slot
+                const int64_t x = max(i, from);
                 while (lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
-                    if (s_row[mid] <= i) lo = mid;
+                    if (s_row[mid] <= x) lo = mid;
                     else hi = mid - 1;
                 }
-                p.slots[i] = slot_of(lo, (int)(i - s_row[lo]));
+                write(i, per, from, to, [&](int64_t i, int &r, int &j) {
+                    while (lo + 1 < nb && s_row[lo + 1] <= i) ++lo;
+                    r = lo;
+                    j = (int)(i - s_row[lo]);
+                    return true;
+                });
             }
             if (s_row[nb] > p.n_slots) err = 1;
         }
@@ -179,11 +217,11 @@ __global__ void __launch_bounds__(kTabThreads) tables_kernel(Tables p)
     }
     if (p.slots) {  // behind the last token
         const int64_t used = p.ld_slots ? (int64_t)p.B * p.ld_slots : rows;
-        for (int64_t i = used + tid; i < p.n_slots; i += kTabThreads) p.slots[i] = -1;
+        for (int64_t i = used + thread; i < p.n_slots; i += threads) p.slots[i] = -1;
     }
-    if (tid == 0) {
-        if (p.row_start) p.row_start[p.B] = (int)min(rows, (int64_t)INT32_MAX);
-        *p.head_out = (int)min((int64_t)p.n_free, (int64_t)head + pages);
+    if (thread == 0) {
+        if (p.row_start) p.row_start[p.B] = clip(rows);
+        if (p.head_out) *p.head_out = (int)min((int64_t)p.n_free, (int64_t)head + pages);
     }
     if (err) atomicOr(p.status, DC_DEVERR_POOL);
 }
@@ -219,49 +257,93 @@ struct Logits {
 };
 
 constexpr uint32_t kSeen = 0x80000000u;
+constexpr int kTile = 4;  // logits of a lane in flight
 
 // One block per chunk of a row's vocabulary: the tokens known so far that
 // fall into the chunk are counted in shared memory (bit 31: seen in the
-// prompt; the rest: how often generated), then the logits stream through.
+// prompt; the rest: how often generated), then the logits stream through, a
+// warp's lanes side by side so that rows of any alignment are read and
+// written in whole lines.  HBM-bound; a larger chunk scans the tokens less
+// often, a smaller one spreads few rows over more SMs.
 template <typename T>
-__global__ void __launch_bounds__(256) logits_kernel(Logits p)
+__global__ void __launch_bounds__(512) logits_kernel(const __grid_constant__ Logits p)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
-    extern __shared__ uint32_t hist[];
+    extern __shared__ __align__(16) uint32_t hist[];
     const int b = blockIdx.x / p.chunks, v0 = blockIdx.x % p.chunks * p.chunk;
-    const int n = min(p.chunk, p.V - v0);
+    const int n = min(p.chunk, p.V - v0);  // chunk: a multiple of 32
     const bool pens = p.rep || p.pres || p.freq;
     if (pens) {
-        for (int i = threadIdx.x; i < n; i += blockDim.x) hist[i] = 0;
-        __syncthreads();
-        const int known = min(p.ldt, p.pos[(int64_t)b * p.pos_stride] + 1);
+        for (int i = threadIdx.x; i < p.chunk / 4; i += blockDim.x)
+            reinterpret_cast<uint4 *>(hist)[i] = make_uint4(0, 0, 0, 0);
+        const int at = p.pos[(int64_t)b * p.pos_stride];
+        const int known = at < 0 ? 0 : min(p.ldt, at + 1);
         const int prompt = p.prompt ? p.prompt[b] : 0;
         const int32_t *tok = p.tokens + (int64_t)b * p.ldt;
-        for (int i = threadIdx.x; i < known; i += blockDim.x) {
-            const uint32_t v = (uint32_t)(tok[i] - v0);
-            if (v < (uint32_t)n) {
-                if (i < prompt) atomicOr(hist + v, kSeen);
-                else atomicAdd(hist + v, 1u);
+        __syncthreads();
+        for (int i0 = threadIdx.x; i0 < known; i0 += 4 * blockDim.x) {
+            int v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = i0 + k * (int)blockDim.x < known ? tok[i0 + k * blockDim.x] : -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t c = (uint32_t)v[k] - (uint32_t)v0;
+                if (v[k] >= 0 && c < (uint32_t)n) {
+                    if (i0 + k * (int)blockDim.x < prompt) atomicOr(hist + c, kSeen);
+                    else atomicAdd(hist + c, 1u);
+                }
             }
         }
         __syncthreads();
     }
-    const float rep = p.rep ? p.rep[b] : 1.f, pres = p.pres ? p.pres[b] : 0.f, freq = p.freq ? p.freq[b] : 0.f;
+    const float rep = p.rep ? p.rep[b] : 1.f, inv = 1.f / rep;
+    const float pres = p.pres ? p.pres[b] : 0.f, freq = p.freq ? p.freq[b] : 0.f;
     const T *in = static_cast<const T *>(p.in) + b * p.ldl + v0;
     T *out = static_cast<T *>(p.out) + b * p.ldo + v0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        float x = to_f<T>(in[i]);
-        const uint32_t h = pens ? hist[i] : 0;
-        if (h) {
-            if (p.rep) x = x > 0.f ? x / rep : x * rep;
-            const uint32_t made = h & ~kSeen;
-            if (made) x = (x - freq * (float)made) - pres;
+    const float *bias = p.bias ? p.bias + b * p.ldb + v0 : nullptr;
+    const uint32_t *mask = p.mask ? p.mask + b * p.ldm + v0 / 32 : nullptr;
+    const int lane = threadIdx.x & 31;
+    auto tile = [&](int t0, auto whole) {  // logits t0 + 32 k + lane
+        const int left = whole ? 32 * kTile : n - t0 - lane;
+        const T *src = in + t0 + lane;
+        T x[kTile];
+        float y[kTile];
+        uint32_t m[kTile], h[kTile];
+#pragma unroll
+        for (int k = 0; k < kTile; ++k) x[k] = whole || 32 * k < left ? src[32 * k] : from_f<T>(0.f);
+        if (bias) {
+            const float *add = bias + t0 + lane;
+#pragma unroll
+            for (int k = 0; k < kTile; ++k) y[k] = whole || 32 * k < left ? add[32 * k] : 0.f;
         }
-        if (p.bias) x += p.bias[b * p.ldb + v0 + i];
-        if (p.mask && !(p.mask[b * p.ldm + (v0 + i) / 32] >> ((v0 + i) & 31) & 1u)) x = -INFINITY;
-        out[i] = from_f<T>(x);
-    }
+        if (mask) {
+            const uint32_t *word = mask + t0 / 32;
+#pragma unroll
+            for (int k = 0; k < kTile; ++k) m[k] = whole || 32 * k < left + lane ? word[k] : 0;
+        }
+        if (pens) {
+            const uint32_t *seen = hist + t0 + lane;
+#pragma unroll
+            for (int k = 0; k < kTile; ++k) h[k] = whole || 32 * k < left ? seen[32 * k] : 0;
+        }
+        T *dst = out + t0 + lane;
+#pragma unroll
+        for (int k = 0; k < kTile; ++k) {
+            float f = to_f<T>(x[k]);
+            if (pens) {
+                const float made = (float)(h[k] & ~kSeen), g = f * (f > 0.f ? inv : rep);
+                if (h[k]) f = g;
+                if (made > 0.f) f = fmaf(-freq, made, f) - pres;
+            }
+            if (bias) f += y[k];
+            if (mask && !(m[k] >> lane & 1u)) f = -INFINITY;
+            if (whole || 32 * k < left) dst[32 * k] = from_f<T>(f);
+        }
+    };
+    int t0 = (threadIdx.x & ~31) * kTile;
+    for (; t0 + 32 * kTile <= n; t0 += blockDim.x * kTile) tile(t0, std::true_type{});
+    if (t0 < n) tile(t0, std::false_type{});
 }
 
 // ------------------------------------------------------------ pick
@@ -277,22 +359,26 @@ struct Pick {
     int ldt;
     float *x;
     int *status;
+    int cluster;  // blocks a row
 };
 
-// One block per row: argmax (lowest index on ties, NaN never wins), the
-// token's embedding at the row's next position, the advanced position.
+// One block per row, or a cluster of them for few long rows: argmax (lowest
+// index on ties, NaN never wins), the token's embedding at the row's next
+// position, the advanced position.  A warp's lanes read side by side, 32
+// bytes each in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) pick_kernel(Pick p)
+__global__ void __launch_bounds__(512) pick_kernel(const __grid_constant__ Pick p)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
-    __shared__ float sv[8];
-    __shared__ int si[8];
-    const int b = blockIdx.x;
+    __shared__ float sv[16];
+    __shared__ int si[16];
+    const int parts = p.cluster, b = blockIdx.x / parts, part = blockIdx.x % parts;
     const int at = p.pos[b];
-    __syncthreads();  // pos_out may be pos: every thread has read its position
-    if (at < 0 || at >= p.ldt - 1) {
-        if (threadIdx.x == 0) {
+    if (parts > 1) cluster_sync_all();  // pos_out may be pos: every thread has read its position
+    else __syncthreads();
+    if (at < 0 || at >= p.ldt - 1) {  // the same in the row's whole cluster
+        if (part == 0 && threadIdx.x == 0) {
             p.pos_out[b] = at;
             if (at >= 0) atomicOr(p.status, DC_DEVERR_FULL);
         }
@@ -300,14 +386,36 @@ __global__ void __launch_bounds__(256) pick_kernel(Pick p)
     }
     const T *l = static_cast<const T *>(p.logits) + b * p.ldl;
     float best = -INFINITY;
-    int bi = 0x7fffffff;
+    int bi = INT_MAX;
+    constexpr int U = 32 / sizeof(T);
+    const int step = U * blockDim.x * parts;
+    auto tile = [&](int64_t v0, auto whole) {  // logits v0 + 32 k, in increasing order
+        const T *src = l + v0;
+        float f[U], top = NAN;
+        T x[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) x[k] = whole || v0 + 32 * k < p.V ? src[32 * k] : from_f<T>(NAN);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            f[k] = to_f<T>(x[k]);
+            top = fmaxf(top, f[k]);  // of the numbers among them
+        }
+        if (top > best || (top == best && bi == INT_MAX)) {
+            best = top;
+#pragma unroll
+            for (int k = U - 1; k >= 0; --k)
+                if (f[k] == top) bi = (int)v0 + 32 * k;
+        }
+    };
+    int64_t v0 = (int64_t)part * U * blockDim.x + (threadIdx.x & ~31) * U + (threadIdx.x & 31);
+    for (; v0 + 32 * (U - 1) < p.V; v0 += step) tile(v0, std::true_type{});
+    if (v0 < p.V) tile(v0, std::false_type{});
     auto take = [&](float x, int v) {
         if (x > best || (x == best && v < bi)) {
             best = x;
             bi = v;
         }
     };
-    for (int v = threadIdx.x; v < p.V; v += blockDim.x) take(to_f<T>(l[v]), v);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -319,7 +427,21 @@ __global__ void __launch_bounds__(256) pick_kernel(Pick p)
         si[threadIdx.x >> 5] = bi;
     }
     __syncthreads();
-    for (int k = 0; k < 8; ++k) take(sv[k], si[k]);
+    for (int k = 0; k < (int)blockDim.x / 32; ++k) take(sv[k], si[k]);
+    if (parts > 1) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sv[0] = best;
+            si[0] = bi;
+        }
+        cluster_sync_all();
+        if (part == 0)
+            for (int k = 1; k < parts; ++k)
+                take(ld_dsmem_f32(smem_in_cta(smem_u32(sv), k)),
+                     __float_as_int(ld_dsmem_f32(smem_in_cta(smem_u32(si), k))));
+        cluster_sync_all();  // the others' shared memory stays until it is read
+        if (part) return;
+    }
     const int tok = bi < p.V ? bi : 0;  // all NaN: token 0
     if (threadIdx.x == 0) {
         p.tokens[(int64_t)b * p.ldt + at + 1] = tok;
@@ -374,7 +496,26 @@ int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_s
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("page_tables", st);
-    DC_CUDA_TRY(launch_pdl(tables_kernel, dim3(1), dim3(kTabThreads), 0, st, 1, p));
+    p.slots4 = aligned16(slots);
+    // One CTA for a decode step or a few prompts (3.6 us for 64 requests of
+    // one token; 148 CTAs 4.5 us); for more tokens a CTA per 4096 slots, or
+    // per 32 requests of new pages, up to one an SM (500 prompts of 1024
+    // tokens: 504 us on one CTA).
+    const int64_t work = std::max<int64_t>(slots ? n_slots : 0, (int64_t)128 * B);
+    const int grid = B <= kTabThreads && (slots ? n_slots : 0) <= 8192
+                         ? 1 : (int)std::min<int64_t>(sm_count(), (work + 4095) / 4096);
+    int last = grid;
+    if (grid > 1 && free_head == free_head_out) {
+        // other CTAs may still have to read the head that one would advance:
+        // a second launch of one CTA does (and writes the same entries again)
+        p.head_out = nullptr;
+        DC_CUDA_TRY(launch_pdl(tables_kernel, dim3(grid), dim3(kTabThreads), 0, st, 1, p));
+        p.head_out = free_head_out;
+        p.slots = nullptr;
+        p.row_start = nullptr;
+        last = 1;
+    }
+    DC_CUDA_TRY(launch_pdl(tables_kernel, dim3(last), dim3(kTabThreads), 0, st, 1, p));
     return DC_OK;
 }
 
@@ -403,7 +544,11 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
     p.ldo = ldo;
     p.B = B;
     p.V = V;
-    p.chunk = 4096;
+    // chunks of 1024 while the grid is short of four blocks an SM, of at most
+    // 16384 (64 KB of counts)
+    const int64_t fill = (4LL * sm_count() + B - 1) / B;
+    const int64_t want = std::max<int64_t>((V + 16383) / 16384, std::min<int64_t>((V + 1023) / 1024, fill));
+    p.chunk = (int)round_up((V + want - 1) / want, 32);
     p.chunks = (V + p.chunk - 1) / p.chunk;
     p.tokens = tokens;
     p.ldt = ldt;
@@ -420,10 +565,14 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
     if ((int64_t)B * p.chunks > INT32_MAX) return fail(DC_ERR_INVALID, "B * V too large");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("logits_controls", st);
-    const dim3 grid((unsigned)(B * p.chunks));
-    const size_t smem = pens ? p.chunk * sizeof(uint32_t) : 0;
-    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(logits_kernel<float>, grid, dim3(256), smem, st, 1, p)
-                                : launch_pdl(logits_kernel<__nv_bfloat16>, grid, dim3(256), smem, st, 1, p));
+    const dim3 grid((unsigned)(B * p.chunks)), block(p.chunk > 4096 ? 512 : 256);
+    const int smem = pens ? p.chunk * (int)sizeof(uint32_t) : 0;
+    auto kernel = dtype == DC_F32 ? logits_kernel<float> : logits_kernel<__nv_bfloat16>;
+    if (smem > 48 * 1024) {
+        static SmemOnce once[2];
+        DC_CUDA_TRY(once[dtype == DC_F32].set(kernel, 64 * 1024));
+    }
+    DC_CUDA_TRY(launch_pdl(kernel, grid, block, smem, st, 1, p));
     return DC_OK;
 }
 
@@ -454,8 +603,12 @@ int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, c
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("greedy_embed_rows", st);
-    DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(pick_kernel<float>, dim3(B), dim3(256), 0, st, 1, p)
-                                : launch_pdl(pick_kernel<__nv_bfloat16>, dim3(B), dim3(256), 0, st, 1, p));
+    // a cluster a row while rows are few and long (one row of 131072 logits:
+    // 8 blocks against 1)
+    p.cluster = V >= 16384 && B <= sm_count() / 4 ? 8 : 1;
+    const dim3 grid((unsigned)(B * p.cluster)), block(V > 2048 ? 512 : 128);
+    auto kernel = dtype == DC_F32 ? pick_kernel<float> : pick_kernel<__nv_bfloat16>;
+    DC_CUDA_TRY(launch_pdl(kernel, grid, block, 0, st, p.cluster, p));
     return DC_OK;
 }
 
