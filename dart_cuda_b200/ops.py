@@ -23,7 +23,8 @@ from ._lib import (DC_AFT_ACCUMULATE, DC_AFT_BWD_DKDV, DC_AFT_BWD_NO_DKDV, DC_AF
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the current stream's handle, without building a Stream object (3 us)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -310,25 +311,28 @@ def gemm(A, B, out=None, trans_a=False, trans_b=False, bias=None, residual=None,
 
 
 # ---------------------------------------------------------------- ragged generation
-def _here(dtype, ndim, **tensors):
+def _here(dtype, ndim, tensors, names):
     """The given tensors (None passes) are CUDA tensors of the current device,
     of one dtype (None: any) and ndim dimensions, with unit stride in the last."""
     dev = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is None:
+    for i, t in enumerate(tensors):
+        if t is None or (t.get_device() == dev and (t.dtype is dtype or dtype is None) and t.dim() == ndim
+                         and (t.is_contiguous() or t.stride()[-1] == 1)):
             continue
-        if not t.is_cuda or t.device.index != dev:
+        name = names.split()[i]
+        if t.get_device() != dev:
             raise DcError(f"{name} must be a CUDA tensor on the current device")
-        if dtype is not None and t.dtype != dtype:
+        if dtype is not None and t.dtype is not dtype:
             raise DcError(f"{name} must be {dtype} (got {t.dtype})")
-        if t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
-            raise DcError(f"{name} must be {ndim}-D with unit stride in the last dimension")
+        raise DcError(f"{name} must be {ndim}-D with unit stride in the last dimension")
 
 
 def _ld2(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor (the width, where there is one row: torch
-    gives such a row any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    """Row stride of a 2-D tensor (at least the width where there is one row:
+    torch gives such a row any stride)."""
+    rows, cols = t.shape
+    ld = t.stride()[0]
+    return ld if rows > 1 else max(ld, cols)
 
 
 def kv4_slab(D: int) -> int:
@@ -347,11 +351,12 @@ def kv4_pages(n_pages: int, page_size: int, D: int, device=None) -> torch.Tensor
 
 def _pool(pages: torch.Tensor, D: int):
     """(n_pages, page_size) of a pool made by kv4_pages for D channels."""
-    _here(torch.uint8, 4, pages=pages)
+    _here(torch.uint8, 4, (pages,), "pages")
     W = kv4_slab(D)
-    if not W or pages.shape[1] * W != D or pages.shape[3] * 4 != 5 * W or not pages.is_contiguous():
+    n_pages, slabs, page_size, record = pages.shape
+    if not W or slabs * W != D or record * 4 != 5 * W or not pages.is_contiguous():
         raise DcError(f"pages must be a contiguous kv4_pages pool of {D} channels (got {tuple(pages.shape)})")
-    return pages.shape[0], pages.shape[2]
+    return n_pages, page_size
 
 
 def page_tables(start, count, free_pages, free_head, table, page_size, slots=None, ld_slots=0, row_start=None,
@@ -364,11 +369,11 @@ def page_tables(start, count, free_pages, free_head, table, page_size, slots=Non
     or with ``ld_slots`` entries a request, -1 elsewhere; ``row_start`` [B+1]
     the prefix sums of the counts.  All int32."""
     head_out = free_head if head_out is None else head_out
-    _here(torch.int32, 1, start=start, count=count, free_pages=free_pages, free_head=free_head, head_out=head_out,
-          slots=slots, row_start=row_start)
-    _here(torch.int32, 2, table=table)
-    B = start.shape[0]
-    if count.shape[0] != B or table.shape[0] != B or (row_start is not None and row_start.shape[0] != B + 1):
+    _here(torch.int32, 1, (start, count, free_pages, free_head, head_out, slots, row_start),
+          "start count free_pages free_head head_out slots row_start")
+    _here(torch.int32, 2, (table,), "table")
+    B, width = table.shape
+    if start.shape[0] != B or count.shape[0] != B or (row_start is not None and row_start.shape[0] != B + 1):
         raise DcError("start, count, table and row_start differ in the number of requests")
     if free_head.shape[0] != 1 or head_out.shape[0] != 1:
         raise DcError("free_head and head_out hold one value")
@@ -376,7 +381,7 @@ def page_tables(start, count, free_pages, free_head, table, page_size, slots=Non
         raise DcError("table must be contiguous")
     check(lib().dc_page_tables(start.data_ptr(), count.data_ptr(), B, int(page_size), free_pages.data_ptr(),
                                free_pages.shape[0], free_head.data_ptr(), head_out.data_ptr(), table.data_ptr(),
-                               table.shape[1], _ptr(slots), 0 if slots is None else slots.shape[0], int(ld_slots),
+                               width, _ptr(slots), 0 if slots is None else slots.shape[0], int(ld_slots),
                                _ptr(row_start), _stream()), "dc_page_tables")
     return slots
 
@@ -387,18 +392,18 @@ def kv4_write(k, v, slots, pages, values=None):
     ``kv4_pages`` pool; rows with a negative slot are left out.  ``values``:
     (k, v) tensors that receive what the stored codes stand for (may be k and
     v themselves)."""
-    _here(k.dtype, 2, k=k, v=v)
-    _here(torch.int32, 1, slots=slots)
-    n, D = k.shape
-    n_pages, page_size = _pool(pages, D)
-    if v.shape != k.shape or slots.shape[0] != n or _ld2(v) != _ld2(k):
-        raise DcError("k, v and slots must have the same rows, k and v the same row stride")
     vk, vv = values if values is not None else (None, None)
+    _here(k.dtype, 2, (k, v, vk, vv), "k v values[0] values[1]")
+    _here(torch.int32, 1, (slots,), "slots")
+    n, D = k.shape
+    ld = _ld2(k)
+    n_pages, page_size = _pool(pages, D)
+    if v.shape != k.shape or slots.shape[0] != n or _ld2(v) != ld:
+        raise DcError("k, v and slots must have the same rows, k and v the same row stride")
     if vk is not None:
-        _here(k.dtype, 2, values_k=vk, values_v=vv)
         if vk.shape != k.shape or vv.shape != k.shape or _ld2(vk) != _ld2(vv):
             raise DcError("values must have the shape of k and one row stride")
-    check(lib().dc_kv4_write(k.data_ptr(), v.data_ptr(), _ld2(k), _dtype_code(k), slots.data_ptr(), n, D,
+    check(lib().dc_kv4_write(k.data_ptr(), v.data_ptr(), ld, _dtype_code(k), slots.data_ptr(), n, D,
                              pages.data_ptr(), n_pages, page_size, _ptr(vk), _ptr(vv),
                              0 if vk is None else _ld2(vk), _stream()), "dc_kv4_write")
     return pages
@@ -416,26 +421,26 @@ def aft_decode4(qkv, w, pages, table, pos, workspace, out=None):
     pos[b] through row b of ``table`` and out[b] is the AFT row over its
     positions 0..pos[b].  w [H, Tmax, Tmax] fp32: the heads' biases.  Rows with
     pos < 0 are left out (their out row is zero)."""
-    _here(None, 2, qkv=qkv)
-    _here(torch.float32, 3, w=w)
-    _here(torch.int32, 2, table=table)
-    _here(torch.int32, 1, pos=pos)
-    _here(torch.uint8, 1, workspace=workspace)
-    B, D = qkv.shape[0], qkv.shape[1] // 3
-    H = w.shape[0]
+    B, D = qkv.shape[0], qkv.shape[-1] // 3
+    z = torch.empty(B, D, dtype=qkv.dtype, device=qkv.device) if out is None else out
+    _here(qkv.dtype, 2, (qkv, z), "qkv out")
+    _here(torch.float32, 3, (w,), "w")
+    _here(torch.int32, 2, (table,), "table")
+    _here(torch.int32, 1, (pos,), "pos")
+    _here(torch.uint8, 1, (workspace,), "workspace")
+    H, rows, cols = w.shape
+    ldh, ldw, _ = w.stride()
     if qkv.shape[1] != 3 * D or H == 0 or D % H:
         raise DcError(f"qkv must be [B, 3D] with D a multiple of the {H} heads (got {tuple(qkv.shape)})")
     if pos.shape[0] != B or table.shape[0] != B or not table.is_contiguous():
         raise DcError("pos and table (contiguous) must have a row per sequence")
     n_pages, page_size = _pool(pages, D)
-    z = torch.empty(B, D, dtype=qkv.dtype, device=qkv.device) if out is None else out
-    _here(qkv.dtype, 2, out=z)
     if z.shape != (B, D):
         raise DcError(f"out must be [{B}, {D}]")
-    check(lib().dc_aft_decode4(qkv.data_ptr(), _ld2(qkv), _dtype_code(qkv), w.data_ptr(), w.stride(1), w.stride(0),
-                               pages.data_ptr(), n_pages, page_size, table.data_ptr(), table.shape[1], B, H, D // H,
-                               pos.data_ptr(), min(w.shape[1], w.shape[2]), z.data_ptr(), _ld2(z),
-                               workspace.data_ptr(), workspace.shape[0], _stream()), "dc_aft_decode4")
+    check(lib().dc_aft_decode4(qkv.data_ptr(), _ld2(qkv), _dtype_code(qkv), w.data_ptr(), ldw if rows > 1 else cols,
+                               ldh, pages.data_ptr(), n_pages, page_size, table.data_ptr(), table.shape[1], B, H,
+                               D // H, pos.data_ptr(), min(rows, cols), z.data_ptr(), _ld2(z), workspace.data_ptr(),
+                               workspace.shape[0], _stream()), "dc_aft_decode4")
     return z
 
 
@@ -448,37 +453,36 @@ def logits_controls(logits, tokens=None, pos=None, prompt_len=None, repetition=N
     presence, frequency: fp32 [B]; bias: fp32 [V] or [B, V]; mask: int32 words
     [ceil(V/32)] or [B, ceil(V/32)], bit v%32 of word v//32 set where token v
     is allowed.  ``out`` may be ``logits``."""
-    _here(None, 2, logits=logits)
-    B, V = logits.shape
     z = torch.empty_like(logits) if out is None else out
-    _here(logits.dtype, 2, out=z)
-    _here(torch.float32, 1, repetition=repetition, presence=presence, frequency=frequency)
-    _here(torch.int32, 1, pos=pos, prompt_len=prompt_len)
-    _here(torch.int32, 2, tokens=tokens)
+    _here(logits.dtype, 2, (logits, z), "logits out")
+    _here(torch.float32, 1, (repetition, presence, frequency), "repetition presence frequency")
+    _here(torch.int32, 1, (pos, prompt_len), "pos prompt_len")
+    _here(torch.int32, 2, (tokens,), "tokens")
+    B, V = logits.shape
     if z.shape != logits.shape:
         raise DcError("out must have the shape of logits")
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency),
-                    ("prompt_len", prompt_len)):
+    for t in (repetition, presence, frequency, prompt_len):
         if t is not None and t.shape[0] != B:
-            raise DcError(f"{name} must hold a value per row")
-    if pos is not None and pos.shape[0] not in (1, B):
+            raise DcError("repetition, presence, frequency and prompt_len must hold a value per row")
+    rows = 0 if pos is None else pos.shape[0]
+    if pos is not None and rows != 1 and rows != B:
         raise DcError("pos must hold one value, or one per row")
     if tokens is not None and (tokens.shape[0] != B or not tokens.is_contiguous()):
         raise DcError("tokens must be contiguous with a row per row of logits")
     ldb = ldm = 0
     if bias is not None:
-        _here(torch.float32, bias.dim() if bias.dim() in (1, 2) else 2, bias=bias)
+        _here(torch.float32, 1 if bias.dim() == 1 else 2, (bias,), "bias")
         if bias.shape[-1] != V or (bias.dim() == 2 and bias.shape[0] != B):
             raise DcError("bias must be [V] or [B, V]")
         ldb = _ld2(bias) if bias.dim() == 2 else 0
     if mask is not None:
-        _here(torch.int32, mask.dim() if mask.dim() in (1, 2) else 2, mask=mask)
+        _here(torch.int32, 1 if mask.dim() == 1 else 2, (mask,), "mask")
         if mask.shape[-1] != (V + 31) // 32 or (mask.dim() == 2 and mask.shape[0] != B):
             raise DcError("mask must be [ceil(V/32)] or [B, ceil(V/32)]")
         ldm = _ld2(mask) if mask.dim() == 2 else 0
     check(lib().dc_logits_controls(logits.data_ptr(), _ld2(logits), z.data_ptr(), _ld2(z), _dtype_code(logits), B, V,
                                    _ptr(tokens), 0 if tokens is None else tokens.shape[1], _ptr(pos),
-                                   int(pos is not None and pos.shape[0] == B), _ptr(prompt_len), _ptr(repetition),
+                                   int(rows == B), _ptr(prompt_len), _ptr(repetition),
                                    _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(mask), ldm, _stream()),
           "dc_logits_controls")
     return z
@@ -489,24 +493,23 @@ def greedy_embed_rows(logits, tokens, pos, wte=None, wpe=None, x=None, pos_out=N
     argmax becomes tokens[b, pos[b]+1], x[b] (when given) the embedding of
     that token at that position, and pos advances (into ``pos_out`` when
     given).  Rows with pos < 0 stay as they are."""
-    _here(None, 2, logits=logits)
     pos_out = pos if pos_out is None else pos_out
-    _here(torch.int32, 2, tokens=tokens)
-    _here(torch.int32, 1, pos=pos, pos_out=pos_out)
-    _here(torch.float32, 2, wte=wte, wpe=wpe, x=x)
+    _here(None, 2, (logits,), "logits")
+    _here(torch.int32, 2, (tokens,), "tokens")
+    _here(torch.int32, 1, (pos, pos_out), "pos pos_out")
+    _here(torch.float32, 2, (wte, wpe, x), "wte wpe x")
     B, V = logits.shape
     D = 0 if x is None else x.shape[1]
+    T = tokens.shape[1]
     if tokens.shape[0] != B or pos.shape[0] != B or pos_out.shape[0] != B or not tokens.is_contiguous():
         raise DcError("tokens (contiguous), pos and pos_out must have a row per row of logits")
     if x is not None:
         if wte is None or wpe is None:
             raise DcError("x needs the embedding tables")
-        if (x.shape[0] != B or wte.shape[0] < V or wte.shape[1] != D or wpe.shape[0] < tokens.shape[1]
-                or wpe.shape[1] != D or not (x.is_contiguous() and wte.is_contiguous() and wpe.is_contiguous())):
+        if (x.shape[0] != B or wte.shape[0] < V or wte.shape[1] != D or wpe.shape[0] < T or wpe.shape[1] != D or not (x.is_contiguous() and wte.is_contiguous() and wpe.is_contiguous())):
             raise DcError("x [B, D], wte [V, D] and wpe [tokens.shape[1], D] must be contiguous")
     check(lib().dc_greedy_embed_rows(logits.data_ptr(), _ld2(logits), _dtype_code(logits), B, V, _ptr(wte), _ptr(wpe),
-                                     pos.data_ptr(), pos_out.data_ptr(), D, tokens.data_ptr(), tokens.shape[1],
-                                     _ptr(x), _stream()), "dc_greedy_embed_rows")
+                                     pos.data_ptr(), pos_out.data_ptr(), D, tokens.data_ptr(), T, _ptr(x), _stream()), "dc_greedy_embed_rows")
     return tokens
 
 
