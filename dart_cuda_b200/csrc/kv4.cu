@@ -477,8 +477,10 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
 // other, are cut into equal shares of q blocks, one share a CTA, so ragged
-// lengths balance and a long sequence spreads over many CTAs.  An item that
-// several CTAs share is merged, in CTA order, by the last of them to finish.
+// lengths balance and a long sequence spreads over many CTAs; or, where that
+// costs little, each item into parts of its own, so that a CTA has one.  An
+// item that several CTAs share is merged, in CTA order, by the last of them
+// to finish.
 template <typename T, int W, int NH>
 __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __grid_constant__ Decode p)
 {
@@ -499,90 +501,97 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     auto part = [&](int warp) { return reinterpret_cast<float *>(ring[warp][0]); };
     static_assert(kStages * kStageBytes >= 8 * 1024, "room for the lanes' sums");
     const uint32_t mine = smem_u32(ring[warp][0]) + sub * (kRows * kRec) + oct * 16;
-    __shared__ int s_sum[kWarps], s_max[kWarps], s_b, s_first, s_t, s_last;
+    __shared__ int s_sum[kWarps], s_max[kWarps], s_active[kWarps], s_b, s_first, s_t, s_last;
 
-    // this CTA's share [u, u1) of the row blocks
-    int sum = 0, most = 0, t = -1, nb = 0, inc = 0;
+    int sum = 0, most = 0, active = 0, t = -1, nb = 0, inc = 0;
     for (int b = tid; b < p.B; b += kThreads) {
         t = p.pos[b];
         nb = row_blocks(p, t);
         sum += nb;
         most = max(most, nb);
+        active += nb > 0;
         if (nb == 0 && b % gridDim.x == blockIdx.x) {  // an inactive sequence
             if (t >= 0) atomicOr(p.status, DC_DEVERR_FULL);
             const float zero[8] = {};
             for (int c = 0; c < p.D; c += 8) store8(static_cast<T *>(p.Z) + b * p.ldz + c, zero);
         }
     }
-    auto scan = [&] {  // inclusive sums of the threads' nb within a warp
-        inc = nb;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    most = __reduce_max_sync(0xffffffffu, most);
+    active = __reduce_add_sync(0xffffffffu, active);
+    if (lane == 0) {
+        s_sum[warp] = sum;
+        s_max[warp] = most;
+        s_active[warp] = active;
+    }
+    if (tid == 0) s_b = -1;
+    __syncthreads();
+    sum = most = active = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+        sum += s_sum[k];
+        most = max(most, s_max[k]);
+        active += s_active[k];
+    }
+    const int64_t total = (int64_t)sum * p.nslab, items = (int64_t)active * p.nslab;
+    const int G = gridDim.x;
+    // at least some rounds of the CTA's warps, so that merging a long sequence's
+    // shares does not outweigh summing them
+    const int least = min(most, kWarps * ((int)sqrtf((float)most) / 8 + 1));
+    int q = (int)max((total + G - 1) / G, (int64_t)least);
+    // even: every item in ceil(nb / q) equal parts of its own, one a CTA, where
+    // that makes no CTA's share much longer (6 blocks cost about what a second
+    // item does: 64 sequences of 256-511 positions, d = 512: 22 -> 14 us)
+    int64_t even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), (int64_t)least) : INT32_MAX;
+    const bool even = even_q <= q + 6;
+    if (even) q = (int)even_q;
+    auto weight = [&](int nb) { return even ? (nb + q - 1) / q : nb; };  // CTAs or blocks of a slab
+    // this CTA's share: [u, u1) of all slabs' weights, one sequence after the other
+    int64_t u = even ? blockIdx.x : (int64_t)blockIdx.x * q;
+    int64_t u1 = even ? u + 1 : min(total, u + q);
+    // the sequence that u lies in: the weight before it
+    const int64_t target = u / p.nslab;
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+        if (p.B > kThreads) {
+            t = b0 + tid < p.B ? p.pos[b0 + tid] : -1;
+            nb = row_blocks(p, t);
+        }
+        const int own = weight(nb);
+        inc = own;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
             const int up = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += up;
         }
-    };
-    scan();
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) {
-        s_sum[warp] = sum;
-        s_max[warp] = most;
-    }
-    if (tid == 0) s_b = -1;
-    __syncthreads();
-    sum = most = 0;
+        __syncthreads();
+        if (lane == 31) s_sum[warp] = inc;
+        __syncthreads();
+        int at = before + inc - own;
 #pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-        sum += s_sum[k];
-        most = max(most, s_max[k]);
-    }
-    const int64_t total = (int64_t)sum * p.nslab;
-    // at least some rounds of the CTA's warps, so that merging a long sequence's
-    // shares does not outweigh summing them
-    const int q = (int)max((total + gridDim.x - 1) / gridDim.x,
-                           (int64_t)min(most, kWarps * ((int)sqrtf((float)most) / 8 + 1)));
-    int64_t u = (int64_t)blockIdx.x * q;
-    const int64_t u1 = min(total, u + q);
-    if (u >= u1) return;
-    // the sequence that unit u lies in: blocks before it, over all sequences
-    const int target = (int)(u / p.nslab);
-    auto locate = [&](int b, int before) {  // before: blocks before this round's
-        int at = before + inc - nb;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k)
+        for (int k = 0; k < kWarps; ++k) {
             if (k < warp) at += s_sum[k];
-        if (target >= at && target < at + nb) {
-            s_b = b;
+            before += s_sum[k];
+        }
+        if (target >= at && target < at + own) {
+            s_b = b0 + tid;
             s_first = at;
             s_t = t;
         }
-    };
-    if (p.B <= kThreads) {
-        locate(tid, 0);
         __syncthreads();
-    } else {
-        int before = 0;
-        for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-            t = b0 + tid < p.B ? p.pos[b0 + tid] : -1;
-            nb = row_blocks(p, t);
-            scan();
-            __syncthreads();
-            if (lane == 31) s_sum[warp] = inc;
-            if (tid == 0) s_b = -1;
-            __syncthreads();
-            locate(b0 + tid, before);
-            __syncthreads();
-            if (s_b >= 0) break;  // target < sum: some sequence holds it
-            for (int k = 0; k < kWarps; ++k) before += s_sum[k];
-        }
+        if (s_b >= 0) break;
     }
     int b = s_b;
-    if (b < 0) return;
+    if (b < 0) return;  // behind the last share
     t = s_t;
     nb = row_blocks(p, t);
-    int slab = (int)((u - (int64_t)s_first * p.nslab) / nb);
-    int blk = (int)((u - (int64_t)s_first * p.nslab) % nb);
+    const int local = (int)(u - (int64_t)s_first * p.nslab), own = weight(nb);
+    int slab = local / own, blk = local % own, j0 = blockIdx.x - blk, j1 = j0 + own - 1;
+    if (even) {  // part blk of own
+        u1 = (int64_t)(blk + 1) * nb / own - (int64_t)blk * nb / own;  // its blocks
+        blk = (int)((int64_t)blk * nb / own);
+        u = 0;
+    }
 
     for (bool first = true;; first = false) {
         const int n = (int)min((int64_t)(nb - blk), u1 - u);
@@ -855,7 +864,10 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             __threadfence();
             __syncthreads();
             const int64_t u_item = u - blk;
-            const int j0 = (int)(u_item / q), j1 = (int)((u_item + nb - 1) / q);
+            if (!even) {
+                j0 = (int)(u_item / q);
+                j1 = (int)((u_item + nb - 1) / q);
+            }
             if (tid == 0) {
                 int *counter = p.counter + (int64_t)b * p.nslab + slab;
                 s_last = atomicAdd(counter, 1) == j1 - j0;
@@ -867,25 +879,30 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 __threadfence();
 #pragma unroll
                 for (int k = 0; k < CPT; ++k) {
-                    const int c = tid + k * kThreads;
-                    if (c >= W) continue;
                     fm[k] = -INFINITY;
                     fn[k] = fd[k] = 0.f;
-                    for (int g0 = j0; g0 <= j1; g0 += 4) {
-                        float x[4][3];
+                }
+                constexpr int kAhead = 8;  // shares whose sums are read at once
+                for (int g0 = j0; g0 <= j1; g0 += kAhead) {
+                    float x[kAhead][CPT][3];
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) {
-                            // the item is CTA g's first unless it begins inside g's share
-                            const int g = min(g0 + d, j1);
-                            const float *src = p.part + ((int64_t)g * 2 + (u_item > (int64_t)g * q)) * 3 * W + c;
-                            x[d][0] = __ldcg(src);
-                            x[d][1] = __ldcg(src + W);
-                            x[d][2] = __ldcg(src + 2 * W);
+                    for (int d = 0; d < kAhead; ++d) {
+                        // the item is CTA g's first unless it begins inside g's share
+                        const int g = min(g0 + d, j1);
+                        const float *src = p.part + ((int64_t)g * 2 + (!even && u_item > (int64_t)g * q)) * 3 * W;
+#pragma unroll
+                        for (int k = 0; k < CPT; ++k) {
+                            const int c = min(tid + k * kThreads, W - 1);
+                            x[d][k][0] = __ldcg(src + c);
+                            x[d][k][1] = __ldcg(src + W + c);
+                            x[d][k][2] = __ldcg(src + 2 * W + c);
                         }
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][0], x[d][1], x[d][2]);
                     }
+#pragma unroll
+                    for (int d = 0; d < kAhead; ++d)
+#pragma unroll
+                        for (int k = 0; k < CPT; ++k)
+                            if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][k][0], x[d][k][1], x[d][k][2]);
                 }
             }
         }
