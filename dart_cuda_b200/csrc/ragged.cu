@@ -364,8 +364,7 @@ struct Pick {
 
 // One block per row, or a cluster of them for few long rows: argmax (lowest
 // index on ties, NaN never wins), the token's embedding at the row's next
-// position, the advanced position.  A warp's lanes read side by side, 32
-// bytes each in flight.
+// position, the advanced position.  64 bytes of a thread are in flight.
 template <typename T>
 __global__ void __launch_bounds__(512) pick_kernel(const __grid_constant__ Pick p)
 {
@@ -387,29 +386,46 @@ __global__ void __launch_bounds__(512) pick_kernel(const __grid_constant__ Pick 
     const T *l = static_cast<const T *>(p.logits) + b * p.ldl;
     float best = -INFINITY;
     int bi = INT_MAX;
-    constexpr int U = 32 / sizeof(T);
-    const int step = U * blockDim.x * parts;
-    auto tile = [&](int64_t v0, auto whole) {  // logits v0 + 32 k, in increasing order
-        const T *src = l + v0;
-        float f[U], top = NAN;
-        T x[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) x[k] = whole || v0 + 32 * k < p.V ? src[32 * k] : from_f<T>(NAN);
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            f[k] = to_f<T>(x[k]);
-            top = fmaxf(top, f[k]);  // of the numbers among them
-        }
-        if (top > best || (top == best && bi == INT_MAX)) {
-            best = top;
-#pragma unroll
-            for (int k = U - 1; k >= 0; --k)
-                if (f[k] == top) bi = (int)v0 + 32 * k;
+    // whole 16-byte vectors, and the logits before and behind them one by one;
+    // a thread meets its logits in increasing order
+    constexpr int N = 16 / sizeof(T), U = 4;
+    const int head = min(p.V, (int)((16 - (reinterpret_cast<uintptr_t>(l) & 15)) % 16 / sizeof(T)));
+    const int vectors = (p.V - head) / N, tail = head + vectors * N;
+    const uint4 *l4 = reinterpret_cast<const uint4 *>(l + head);
+    auto single = [&](int v) {
+        const float f = to_f<T>(l[v]);
+        if (f > best || (f == best && bi == INT_MAX)) {
+            best = f;
+            bi = v;
         }
     };
-    int64_t v0 = (int64_t)part * U * blockDim.x + (threadIdx.x & ~31) * U + (threadIdx.x & 31);
-    for (; v0 + 32 * (U - 1) < p.V; v0 += step) tile(v0, std::true_type{});
-    if (v0 < p.V) tile(v0, std::false_type{});
+    if (part == 0 && (int)threadIdx.x < head) single(threadIdx.x);
+    const int step = blockDim.x * parts;
+    for (int64_t i0 = part * blockDim.x + threadIdx.x; i0 < vectors; i0 += U * step) {
+        uint4 x[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int64_t i = i0 + k * step;
+            x[k] = l4[i < vectors ? i : i0];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const T *e = reinterpret_cast<const T *>(&x[k]);
+            float f[N], top = NAN;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                f[j] = to_f<T>(e[j]);
+                top = fmaxf(top, f[j]);  // of the numbers among them
+            }
+            if (top > best || (top == best && bi == INT_MAX)) {  // a vector read again brings nothing
+                best = top;
+#pragma unroll
+                for (int j = N - 1; j >= 0; --j)
+                    if (f[j] == top) bi = head + (int)(i0 + k * step) * N + j;
+            }
+        }
+    }
+    if (part == 0 && tail + (int)threadIdx.x < p.V) single(tail + threadIdx.x);
     auto take = [&](float x, int v) {
         if (x > best || (x == best && v < bi)) {
             best = x;

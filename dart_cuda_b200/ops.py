@@ -311,15 +311,19 @@ def gemm(A, B, out=None, trans_a=False, trans_b=False, bias=None, residual=None,
 
 
 # ---------------------------------------------------------------- ragged generation
-def _here(dtype, ndim, tensors, names):
-    """The given tensors (None passes) are CUDA tensors of the current device,
-    of one dtype (None: any) and ndim dimensions, with unit stride in the last."""
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
+
+
+def _here(names, *specs):
+    """Each (tensor, dtype, ndim) is a CUDA tensor of the current device, of
+    that dtype (None: any) and number of dimensions, with unit stride in the
+    last; a tensor of None passes."""
     dev = torch.cuda.current_device()
-    for i, t in enumerate(tensors):
+    for t, dtype, ndim in specs:
         if t is None or (t.get_device() == dev and (t.dtype is dtype or dtype is None) and t.dim() == ndim
                          and (t.is_contiguous() or t.stride()[-1] == 1)):
             continue
-        name = names.split()[i]
+        name = names.split()[[s[0] is t for s in specs].index(True)]
         if t.get_device() != dev:
             raise DcError(f"{name} must be a CUDA tensor on the current device")
         if dtype is not None and t.dtype is not dtype:
@@ -351,7 +355,7 @@ def kv4_pages(n_pages: int, page_size: int, D: int, device=None) -> torch.Tensor
 
 def _pool(pages: torch.Tensor, D: int):
     """(n_pages, page_size) of a pool made by kv4_pages for D channels."""
-    _here(torch.uint8, 4, (pages,), "pages")
+    _here("pages", (pages, _U8, 4))
     W = kv4_slab(D)
     n_pages, slabs, page_size, record = pages.shape
     if not W or slabs * W != D or record * 4 != 5 * W or not pages.is_contiguous():
@@ -369,9 +373,9 @@ def page_tables(start, count, free_pages, free_head, table, page_size, slots=Non
     or with ``ld_slots`` entries a request, -1 elsewhere; ``row_start`` [B+1]
     the prefix sums of the counts.  All int32."""
     head_out = free_head if head_out is None else head_out
-    _here(torch.int32, 1, (start, count, free_pages, free_head, head_out, slots, row_start),
-          "start count free_pages free_head head_out slots row_start")
-    _here(torch.int32, 2, (table,), "table")
+    _here("start count free_pages free_head head_out slots row_start table", (start, _I32, 1), (count, _I32, 1),
+          (free_pages, _I32, 1), (free_head, _I32, 1), (head_out, _I32, 1), (slots, _I32, 1), (row_start, _I32, 1),
+          (table, _I32, 2))
     B, width = table.shape
     if start.shape[0] != B or count.shape[0] != B or (row_start is not None and row_start.shape[0] != B + 1):
         raise DcError("start, count, table and row_start differ in the number of requests")
@@ -393,8 +397,9 @@ def kv4_write(k, v, slots, pages, values=None):
     (k, v) tensors that receive what the stored codes stand for (may be k and
     v themselves)."""
     vk, vv = values if values is not None else (None, None)
-    _here(k.dtype, 2, (k, v, vk, vv), "k v values[0] values[1]")
-    _here(torch.int32, 1, (slots,), "slots")
+    dtype = k.dtype
+    _here("k v values[0] values[1] slots", (k, dtype, 2), (v, dtype, 2), (vk, dtype, 2), (vv, dtype, 2),
+          (slots, _I32, 1))
     n, D = k.shape
     ld = _ld2(k)
     n_pages, page_size = _pool(pages, D)
@@ -423,11 +428,8 @@ def aft_decode4(qkv, w, pages, table, pos, workspace, out=None):
     pos < 0 are left out (their out row is zero)."""
     B, D = qkv.shape[0], qkv.shape[-1] // 3
     z = torch.empty(B, D, dtype=qkv.dtype, device=qkv.device) if out is None else out
-    _here(qkv.dtype, 2, (qkv, z), "qkv out")
-    _here(torch.float32, 3, (w,), "w")
-    _here(torch.int32, 2, (table,), "table")
-    _here(torch.int32, 1, (pos,), "pos")
-    _here(torch.uint8, 1, (workspace,), "workspace")
+    _here("qkv out w table pos workspace", (qkv, None, 2), (z, qkv.dtype, 2), (w, _F32, 3), (table, _I32, 2),
+          (pos, _I32, 1), (workspace, _U8, 1))
     H, rows, cols = w.shape
     ldh, ldw, _ = w.stride()
     if qkv.shape[1] != 3 * D or H == 0 or D % H:
@@ -454,10 +456,10 @@ def logits_controls(logits, tokens=None, pos=None, prompt_len=None, repetition=N
     [ceil(V/32)] or [B, ceil(V/32)], bit v%32 of word v//32 set where token v
     is allowed.  ``out`` may be ``logits``."""
     z = torch.empty_like(logits) if out is None else out
-    _here(logits.dtype, 2, (logits, z), "logits out")
-    _here(torch.float32, 1, (repetition, presence, frequency), "repetition presence frequency")
-    _here(torch.int32, 1, (pos, prompt_len), "pos prompt_len")
-    _here(torch.int32, 2, (tokens,), "tokens")
+    _here("logits out tokens pos prompt_len repetition presence frequency bias mask", (logits, None, 2),
+          (z, logits.dtype, 2), (tokens, _I32, 2), (pos, _I32, 1), (prompt_len, _I32, 1), (repetition, _F32, 1),
+          (presence, _F32, 1), (frequency, _F32, 1), (bias, _F32, 1 if bias is None or bias.dim() == 1 else 2),
+          (mask, _I32, 1 if mask is None or mask.dim() == 1 else 2))
     B, V = logits.shape
     if z.shape != logits.shape:
         raise DcError("out must have the shape of logits")
@@ -471,12 +473,10 @@ def logits_controls(logits, tokens=None, pos=None, prompt_len=None, repetition=N
         raise DcError("tokens must be contiguous with a row per row of logits")
     ldb = ldm = 0
     if bias is not None:
-        _here(torch.float32, 1 if bias.dim() == 1 else 2, (bias,), "bias")
         if bias.shape[-1] != V or (bias.dim() == 2 and bias.shape[0] != B):
             raise DcError("bias must be [V] or [B, V]")
         ldb = _ld2(bias) if bias.dim() == 2 else 0
     if mask is not None:
-        _here(torch.int32, 1 if mask.dim() == 1 else 2, (mask,), "mask")
         if mask.shape[-1] != (V + 31) // 32 or (mask.dim() == 2 and mask.shape[0] != B):
             raise DcError("mask must be [ceil(V/32)] or [B, ceil(V/32)]")
         ldm = _ld2(mask) if mask.dim() == 2 else 0
@@ -494,10 +494,8 @@ def greedy_embed_rows(logits, tokens, pos, wte=None, wpe=None, x=None, pos_out=N
     that token at that position, and pos advances (into ``pos_out`` when
     given).  Rows with pos < 0 stay as they are."""
     pos_out = pos if pos_out is None else pos_out
-    _here(None, 2, (logits,), "logits")
-    _here(torch.int32, 2, (tokens,), "tokens")
-    _here(torch.int32, 1, (pos, pos_out), "pos pos_out")
-    _here(torch.float32, 2, (wte, wpe, x), "wte wpe x")
+    _here("logits tokens pos pos_out wte wpe x", (logits, None, 2), (tokens, _I32, 2), (pos, _I32, 1),
+          (pos_out, _I32, 1), (wte, _F32, 2), (wpe, _F32, 2), (x, _F32, 2))
     B, V = logits.shape
     D = 0 if x is None else x.shape[1]
     T = tokens.shape[1]
