@@ -364,6 +364,7 @@ __device__ __forceinline__ float fmax_nan(float a, float b)
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 3;
 constexpr int kRows = 16;  // history rows of a block: two halves, each within a page
 constexpr int kStages = 3;  // blocks in flight of a warp
+constexpr int kItem = 10;   // what an item costs a CTA besides its blocks, in blocks
 
 // 16 bytes, of which the first `bytes` (0 or 16) are read, the others zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes)
@@ -534,21 +535,24 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         active += s_active[k];
     }
     const int64_t total = (int64_t)sum * p.nslab, items = (int64_t)active * p.nslab;
+    const int64_t units = total + items * kItem;
     const int G = gridDim.x;
     // at least some rounds of the CTA's warps, so that merging a long sequence's
     // shares does not outweigh summing them
     const int least = min(most, kWarps * ((int)sqrtf((float)most) / 8 + 1));
-    int q = (int)max((total + G - 1) / G, (int64_t)least);
+    int q = (int)max((units + G - 1) / G, (int64_t)least);
     // even: every item in ceil(nb / q) equal parts of its own, one a CTA, where
-    // that makes no CTA's share much longer (6 blocks cost about what a second
-    // item does: 64 sequences of 256-511 positions, d = 512: 22 -> 14 us)
+    // that makes no CTA's share longer (64 sequences of 256-511 positions,
+    // d = 512: 22 -> 16.7 us)
     int64_t even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), (int64_t)least) : INT32_MAX;
     const bool even = even_q <= q + 6;
     if (even) q = (int)even_q;
-    auto weight = [&](int nb) { return even ? (nb + q - 1) / q : nb; };  // CTAs or blocks of a slab
+    auto weight = [&](int nb) {  // CTAs, or blocks and what an item costs besides
+        return even ? (nb + q - 1) / q : nb ? nb + kItem : 0;
+    };
     // this CTA's share: [u, u1) of all slabs' weights, one sequence after the other
     int64_t u = even ? blockIdx.x : (int64_t)blockIdx.x * q;
-    int64_t u1 = even ? u + 1 : min(total, u + q);
+    int64_t u1 = even ? u + 1 : min(units, u + q);
     // the sequence that u lies in: the weight before it
     const int64_t target = u / p.nslab;
     int before = 0;
@@ -586,15 +590,19 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     t = s_t;
     nb = row_blocks(p, t);
     const int local = (int)(u - (int64_t)s_first * p.nslab), own = weight(nb);
-    int slab = local / own, blk = local % own, j0 = blockIdx.x - blk, j1 = j0 + own - 1;
-    if (even) {  // part blk of own
-        u1 = (int64_t)(blk + 1) * nb / own - (int64_t)blk * nb / own;  // its blocks
-        blk = (int)((int64_t)blk * nb / own);
-        u = 0;
+    int slab = local / own, off = local % own;  // off: units of the item before the share
+    int j0 = blockIdx.x - off, j1 = j0 + own - 1;
+    if (even) {  // part off of own: its blocks, as units behind the item's kItem
+        u1 = kItem + (int64_t)(off + 1) * nb / own;
+        off = kItem + (int)((int64_t)off * nb / own);
+        u = off;
     }
 
-    for (bool first = true;; first = false) {
-        const int n = (int)min((int64_t)(nb - blk), u1 - u);
+    for (;;) {
+        const int taken = (int)min((int64_t)(nb + kItem - off), u1 - u);
+        const int blk = max(0, off - kItem), n = off + taken - kItem - blk;  // the share's blocks
+        const int64_t u_item = u - off;
+        if (n > 0) {
         const int32_t *tab = p.table + b * p.ldtab;
         const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + slab * W;
         const float *w[NH];  // bias rows of this lane's octets
@@ -852,7 +860,9 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         }
         bool finish = n == nb;
         if (!finish) {  // shared with other CTAs
-            float *mine = p.part + ((int64_t)blockIdx.x * 2 + !first) * 3 * W;
+            // second slot: an item that begins inside the CTA's share
+            const auto slot = [&](int g) { return (int64_t)g * 2 + (!even && u_item > (int64_t)g * q); };
+            float *mine = p.part + slot(blockIdx.x) * 3 * W;
 #pragma unroll
             for (int k = 0; k < CPT; ++k) {
                 const int c = tid + k * kThreads;
@@ -863,10 +873,9 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             }
             __threadfence();
             __syncthreads();
-            const int64_t u_item = u - blk;
             if (!even) {
-                j0 = (int)(u_item / q);
-                j1 = (int)((u_item + nb - 1) / q);
+                j0 = (int)((u_item + kItem) / q);
+                j1 = (int)((u_item + kItem + nb - 1) / q);
             }
             if (tid == 0) {
                 int *counter = p.counter + (int64_t)b * p.nslab + slab;
@@ -887,9 +896,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                     float x[kAhead][CPT][3];
 #pragma unroll
                     for (int d = 0; d < kAhead; ++d) {
-                        // the item is CTA g's first unless it begins inside g's share
-                        const int g = min(g0 + d, j1);
-                        const float *src = p.part + ((int64_t)g * 2 + (!even && u_item > (int64_t)g * q)) * 3 * W;
+                        const float *src = p.part + slot(min(g0 + d, j1)) * 3 * W;
 #pragma unroll
                         for (int k = 0; k < CPT; ++k) {
                             const int c = min(tid + k * kThreads, W - 1);
@@ -930,9 +937,10 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                     from_f<T>(fd[k] == 0.f ? 0.f : sigm(qv) * (fn[k] / fd[k]));
             }
         }
-        u += n;
+        }
+        u += taken;
         if (u >= u1) return;
-        blk = 0;
+        off = 0;
         if (++slab == p.nslab) {
             slab = 0;
             do {  // u < total: there is another active one
@@ -1100,7 +1108,7 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     p.ldz = ldz;
     p.status = device_status_word();
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
-    if ((int64_t)B * (p.cap / kRows + 1) > INT32_MAX || (int64_t)B * p.nslab > INT32_MAX / 4)
+    if ((int64_t)B * (p.cap / kRows + 1 + kItem) > INT32_MAX || (int64_t)B * p.nslab > INT32_MAX / 4)
         return fail(DC_ERR_INVALID, "B * Tmax or B * D too large");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("aft_decode4", st);
