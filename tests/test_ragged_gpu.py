@@ -303,6 +303,19 @@ def test_aft_decode4_many_sequences(ops):
     assert torch.count_nonzero(z[[0, 17, 398]]) == 0
 
 
+@pytest.mark.parametrize("B,H,hs,T,page,dtype", [(40, 24, 64, 120, 16, "f32"), (50, 5, 128, 90, 8, "bf16"),
+                                                 (80, 14, 32, 60, 64, "f32"), (36, 32, 24, 70, 8, "f32"),
+                                                 (150, 2, 128, 130, 32, "f32")])
+def test_aft_decode4_uneven_shares(ops, B, H, hs, T, page, dtype):
+    """More (sequence, slab) items than parts of their own would fit: shares
+    that begin and end inside items, of lengths from one position up."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(0, T, B)
+    lens[rng.random(B) < 0.3] = rng.integers(0, 4)
+    lens[[0, B - 1]] = T - 1, -1
+    History(ops, rng, B, H, hs, T, page, dtype, lens).check()
+
+
 def test_aft_decode4_inactive_and_full(ops):
     rng = np.random.default_rng(4)
     h = History(ops, rng, 4, 2, 32, 24, 8, "f32", [-1, 24, 23, -2**31])
