@@ -13,7 +13,7 @@
 // whatever its offset, and code = floor((x - low) / step + 1/2), decided
 // exactly: x >= low + step (c + 1/2) holds in real numbers iff it holds
 // against that border rounded up to fp32 (x is an fp32 number).  |x - value|
-// <= step / 2.  A group with a value that is not finite (or above 1e38 in
+// <= step / 2.  A group with a value that is not finite (or above 1e37 in
 // magnitude) is stored with a NaN step: all its channels read as NaN.
 //
 // The decode step is dc_aft_decode's row t of AFT-full
@@ -37,7 +37,7 @@
 namespace dc {
 namespace kv4 {
 
-constexpr float kBig = 1e38f;        // larger magnitudes count as not finite
+constexpr float kBig = 1e37f;        // larger magnitudes count as not finite
 constexpr int DC_DEVERR_FULL = 0x40;  // a position past the capacity
 constexpr int DC_DEVERR_PAGE = 0x200; // a slot or page id outside the pool
 constexpr float kLog2e = 1.4426950408889634f;
@@ -340,8 +340,8 @@ struct Decode {
     void *Z;
     int64_t ldz;
     int *status;
-    int *counter;  // [B * nslab], zero between launches
     float *part;   // [gridDim.x][2][3][W]
+    int *counter;  // [B * nslab], zero between launches
 };
 
 __device__ __forceinline__ float sigm(float q) { return 1.0f / (1.0f + __expf(-q)); }
@@ -954,6 +954,10 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
 
 static int decode_grid() { return kResident * sm_count(); }
 
+// Partial sums come first, in room for the widest slab, then the counters: a
+// workspace serves calls of any smaller batch or width in between.
+static size_t part_bytes() { return (size_t)decode_grid() * 2 * 3 * 256 * sizeof(float); }
+
 template <typename T, int W>
 static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
 {
@@ -1055,7 +1059,8 @@ size_t dc_aft_decode4_workspace_size(int B, int D)
 {
     const int W = D > 0 ? kv4::slab_width(D) : 0;
     if (B <= 0 || !W) return 0;
-    return round_up((int64_t)B * (D / W) * sizeof(int), 256) + (size_t)kv4::decode_grid() * 2 * 3 * W * sizeof(float);
+    // counters for the narrowest slabs: the size grows with B and D
+    return kv4::part_bytes() + round_up((int64_t)B * (D / 32) * sizeof(int), 256);
 }
 
 int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw, long long head_stride_w,
@@ -1101,9 +1106,8 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     for (p.shift = 3; 1 << p.shift < page_size;) ++p.shift;
     p.page_bytes = (uint32_t)(page_size * (int64_t)D * 5 / 4);
     p.w4 = aligned16(w) && ldw % 4 == 0 && head_stride_w % 4 == 0;
-    p.counter = static_cast<int *>(workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                       round_up((int64_t)B * p.nslab * sizeof(int), 256));
+    p.part = static_cast<float *>(workspace);
+    p.counter = reinterpret_cast<int *>(static_cast<char *>(workspace) + part_bytes());
     p.Z = Z;
     p.ldz = ldz;
     p.status = device_status_word();

@@ -315,12 +315,12 @@ _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
 def _here(names, *specs):
-    """Each (tensor, dtype, ndim) is a CUDA tensor of the current device, of
-    that dtype (None: any) and number of dimensions, with unit stride in the
-    last; a tensor of None passes."""
+    """The current stream, once each (tensor, dtype, ndim) is a CUDA tensor of
+    the current device, of that dtype (None: any) and number of dimensions,
+    with unit stride in the last; a tensor of None passes."""
     dev = torch.cuda.current_device()
     for t, dtype, ndim in specs:
-        if t is None or (t.get_device() == dev and (t.dtype is dtype or dtype is None) and t.dim() == ndim
+        if t is None or (t.dim() == ndim and (t.dtype is dtype or dtype is None) and t.get_device() == dev
                          and (t.is_contiguous() or t.stride()[-1] == 1)):
             continue
         name = names.split()[[s[0] is t for s in specs].index(True)]
@@ -329,6 +329,7 @@ def _here(names, *specs):
         if dtype is not None and t.dtype is not dtype:
             raise DcError(f"{name} must be {dtype} (got {t.dtype})")
         raise DcError(f"{name} must be {ndim}-D with unit stride in the last dimension")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _ld2(t: torch.Tensor) -> int:
@@ -373,9 +374,9 @@ def page_tables(start, count, free_pages, free_head, table, page_size, slots=Non
     or with ``ld_slots`` entries a request, -1 elsewhere; ``row_start`` [B+1]
     the prefix sums of the counts.  All int32."""
     head_out = free_head if head_out is None else head_out
-    _here("start count free_pages free_head head_out slots row_start table", (start, _I32, 1), (count, _I32, 1),
-          (free_pages, _I32, 1), (free_head, _I32, 1), (head_out, _I32, 1), (slots, _I32, 1), (row_start, _I32, 1),
-          (table, _I32, 2))
+    st = _here("start count free_pages free_head head_out slots row_start table", (start, _I32, 1), (count, _I32, 1),
+               (free_pages, _I32, 1), (free_head, _I32, 1), (head_out, _I32, 1), (slots, _I32, 1), (row_start, _I32, 1),
+               (table, _I32, 2))
     B, width = table.shape
     if start.shape[0] != B or count.shape[0] != B or (row_start is not None and row_start.shape[0] != B + 1):
         raise DcError("start, count, table and row_start differ in the number of requests")
@@ -386,7 +387,7 @@ def page_tables(start, count, free_pages, free_head, table, page_size, slots=Non
     check(lib().dc_page_tables(start.data_ptr(), count.data_ptr(), B, int(page_size), free_pages.data_ptr(),
                                free_pages.shape[0], free_head.data_ptr(), head_out.data_ptr(), table.data_ptr(),
                                width, _ptr(slots), 0 if slots is None else slots.shape[0], int(ld_slots),
-                               _ptr(row_start), _stream()), "dc_page_tables")
+                               _ptr(row_start), st), "dc_page_tables")
     return slots
 
 
@@ -398,8 +399,8 @@ def kv4_write(k, v, slots, pages, values=None):
     v themselves)."""
     vk, vv = values if values is not None else (None, None)
     dtype = k.dtype
-    _here("k v values[0] values[1] slots", (k, dtype, 2), (v, dtype, 2), (vk, dtype, 2), (vv, dtype, 2),
-          (slots, _I32, 1))
+    st = _here("k v values[0] values[1] slots", (k, dtype, 2), (v, dtype, 2), (vk, dtype, 2), (vv, dtype, 2),
+               (slots, _I32, 1))
     n, D = k.shape
     ld = _ld2(k)
     n_pages, page_size = _pool(pages, D)
@@ -410,13 +411,13 @@ def kv4_write(k, v, slots, pages, values=None):
             raise DcError("values must have the shape of k and one row stride")
     check(lib().dc_kv4_write(k.data_ptr(), v.data_ptr(), ld, _dtype_code(k), slots.data_ptr(), n, D,
                              pages.data_ptr(), n_pages, page_size, _ptr(vk), _ptr(vv),
-                             0 if vk is None else _ld2(vk), _stream()), "dc_kv4_write")
+                             0 if vk is None else _ld2(vk), st), "dc_kv4_write")
     return pages
 
 
 def aft_decode4_workspace(B: int, D: int, device=None) -> torch.Tensor:
-    """Zeroed workspace of aft_decode4 for B sequences of D channels; calls
-    that may overlap on the GPU need one each."""
+    """Zeroed workspace of aft_decode4 for up to B sequences of up to D
+    channels; calls that may overlap on the GPU need one each."""
     return torch.zeros(lib().dc_aft_decode4_workspace_size(int(B), int(D)), dtype=torch.uint8, device=device or "cuda")
 
 
@@ -428,8 +429,8 @@ def aft_decode4(qkv, w, pages, table, pos, workspace, out=None):
     pos < 0 are left out (their out row is zero)."""
     B, D = qkv.shape[0], qkv.shape[-1] // 3
     z = torch.empty(B, D, dtype=qkv.dtype, device=qkv.device) if out is None else out
-    _here("qkv out w table pos workspace", (qkv, None, 2), (z, qkv.dtype, 2), (w, _F32, 3), (table, _I32, 2),
-          (pos, _I32, 1), (workspace, _U8, 1))
+    st = _here("qkv out w table pos workspace", (qkv, None, 2), (z, qkv.dtype, 2), (w, _F32, 3), (table, _I32, 2),
+               (pos, _I32, 1), (workspace, _U8, 1))
     H, rows, cols = w.shape
     ldh, ldw, _ = w.stride()
     if qkv.shape[1] != 3 * D or H == 0 or D % H:
@@ -442,7 +443,7 @@ def aft_decode4(qkv, w, pages, table, pos, workspace, out=None):
     check(lib().dc_aft_decode4(qkv.data_ptr(), _ld2(qkv), _dtype_code(qkv), w.data_ptr(), ldw if rows > 1 else cols,
                                ldh, pages.data_ptr(), n_pages, page_size, table.data_ptr(), table.shape[1], B, H,
                                D // H, pos.data_ptr(), min(rows, cols), z.data_ptr(), _ld2(z), workspace.data_ptr(),
-                               workspace.shape[0], _stream()), "dc_aft_decode4")
+                               workspace.shape[0], st), "dc_aft_decode4")
     return z
 
 
@@ -456,10 +457,10 @@ def logits_controls(logits, tokens=None, pos=None, prompt_len=None, repetition=N
     [ceil(V/32)] or [B, ceil(V/32)], bit v%32 of word v//32 set where token v
     is allowed.  ``out`` may be ``logits``."""
     z = torch.empty_like(logits) if out is None else out
-    _here("logits out tokens pos prompt_len repetition presence frequency bias mask", (logits, None, 2),
-          (z, logits.dtype, 2), (tokens, _I32, 2), (pos, _I32, 1), (prompt_len, _I32, 1), (repetition, _F32, 1),
-          (presence, _F32, 1), (frequency, _F32, 1), (bias, _F32, 1 if bias is None or bias.dim() == 1 else 2),
-          (mask, _I32, 1 if mask is None or mask.dim() == 1 else 2))
+    st = _here("logits out tokens pos prompt_len repetition presence frequency bias mask", (logits, None, 2),
+               (z, logits.dtype, 2), (tokens, _I32, 2), (pos, _I32, 1), (prompt_len, _I32, 1), (repetition, _F32, 1),
+               (presence, _F32, 1), (frequency, _F32, 1), (bias, _F32, 1 if bias is None or bias.dim() == 1 else 2),
+               (mask, _I32, 1 if mask is None or mask.dim() == 1 else 2))
     B, V = logits.shape
     if z.shape != logits.shape:
         raise DcError("out must have the shape of logits")
@@ -481,10 +482,9 @@ def logits_controls(logits, tokens=None, pos=None, prompt_len=None, repetition=N
             raise DcError("mask must be [ceil(V/32)] or [B, ceil(V/32)]")
         ldm = _ld2(mask) if mask.dim() == 2 else 0
     check(lib().dc_logits_controls(logits.data_ptr(), _ld2(logits), z.data_ptr(), _ld2(z), _dtype_code(logits), B, V,
-                                   _ptr(tokens), 0 if tokens is None else tokens.shape[1], _ptr(pos),
-                                   int(rows == B), _ptr(prompt_len), _ptr(repetition),
-                                   _ptr(presence), _ptr(frequency), _ptr(bias), ldb, _ptr(mask), ldm, _stream()),
-          "dc_logits_controls")
+                                   _ptr(tokens), 0 if tokens is None else tokens.shape[1], _ptr(pos), int(rows == B),
+                                   _ptr(prompt_len), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias),
+                                   ldb, _ptr(mask), ldm, st), "dc_logits_controls")
     return z
 
 
@@ -494,8 +494,8 @@ def greedy_embed_rows(logits, tokens, pos, wte=None, wpe=None, x=None, pos_out=N
     that token at that position, and pos advances (into ``pos_out`` when
     given).  Rows with pos < 0 stay as they are."""
     pos_out = pos if pos_out is None else pos_out
-    _here("logits tokens pos pos_out wte wpe x", (logits, None, 2), (tokens, _I32, 2), (pos, _I32, 1),
-          (pos_out, _I32, 1), (wte, _F32, 2), (wpe, _F32, 2), (x, _F32, 2))
+    st = _here("logits tokens pos pos_out wte wpe x", (logits, None, 2), (tokens, _I32, 2), (pos, _I32, 1),
+               (pos_out, _I32, 1), (wte, _F32, 2), (wpe, _F32, 2), (x, _F32, 2))
     B, V = logits.shape
     D = 0 if x is None else x.shape[1]
     T = tokens.shape[1]
@@ -504,10 +504,12 @@ def greedy_embed_rows(logits, tokens, pos, wte=None, wpe=None, x=None, pos_out=N
     if x is not None:
         if wte is None or wpe is None:
             raise DcError("x needs the embedding tables")
-        if (x.shape[0] != B or wte.shape[0] < V or wte.shape[1] != D or wpe.shape[0] < T or wpe.shape[1] != D or not (x.is_contiguous() and wte.is_contiguous() and wpe.is_contiguous())):
+        if (x.shape[0] != B or wte.shape[0] < V or wte.shape[1] != D or wpe.shape[0] < T or wpe.shape[1] != D
+                or not (x.is_contiguous() and wte.is_contiguous() and wpe.is_contiguous())):
             raise DcError("x [B, D], wte [V, D] and wpe [tokens.shape[1], D] must be contiguous")
     check(lib().dc_greedy_embed_rows(logits.data_ptr(), _ld2(logits), _dtype_code(logits), B, V, _ptr(wte), _ptr(wpe),
-                                     pos.data_ptr(), pos_out.data_ptr(), D, tokens.data_ptr(), T, _ptr(x), _stream()), "dc_greedy_embed_rows")
+                                     pos.data_ptr(), pos_out.data_ptr(), D, tokens.data_ptr(), T, _ptr(x), st),
+          "dc_greedy_embed_rows")
     return tokens
 
 

@@ -337,7 +337,7 @@ int dc_kv_cache_fill(const float *qkv, int ldq, int B, int T, int D, float *cach
  * entries of slots [n_slots] that belong to no token become -1.  row_start
  * [B + 1] receives the prefix sums of the counts.  slots and row_start may be
  * NULL.  A token for which there is no page left gets -1 and sets status bit
- * 0x100.  page_size: 8, 16, 32, 64, 128 or 256. */
+ * 0x100.  page_size: 8, 16, 32, 64, 128 or 256.  B = 0 does nothing. */
 int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_size,
                    const int32_t *free_pages, int n_free, const int32_t *free_head,
                    int32_t *free_head_out, int32_t *table, int ldtab, int32_t *slots, int n_slots,
@@ -352,7 +352,7 @@ int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_s
  * low the largest bf16 <= the group's minimum, step the smallest bf16 >=
  * (maximum - low) / 15 and c = floor((x - low) / step + 1/2), so a value is
  * off by at most step / 2.  A group with a value that is not finite, or
- * above 1e38 in magnitude, reads as NaN.
+ * above 1e37 in magnitude, reads as NaN.
  *
  * dc_kv4_write quantises n rows of k and v (row stride ld, `dtype`, 16-byte
  * aligned rows) into the slots slots[n]; rows whose slot is negative are left
@@ -375,7 +375,8 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
  * whose bias row is -inf throughout.  Sequences may share pages they only
  * read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
  * zero-filled once before its first use (the kernel leaves its counters
- * zeroed); calls that may overlap on the GPU need one each. */
+ * zeroed), for this or any smaller B and D; calls that may overlap on the GPU
+ * need one each. */
 size_t dc_aft_decode4_workspace_size(int B, int D);
 int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
                    long long head_stride_w, void *pages, int n_pages, int page_size,

@@ -47,7 +47,7 @@ def quantise_group(x):
     """(codes, step, low) of 32 fp32 values, in exact arithmetic; None for the
     codes of a group that is stored as NaN."""
     x = np.asarray(x, np.float32)
-    if not np.all(np.abs(x) <= np.float32(1e38)):
+    if not np.all(np.abs(x) <= np.float32(1e37)):
         return None, np.float32(np.nan), np.float32(0)
     low = bf16_floor(x.min())
     step = bf16_ceil((Fraction(float(x.max())) - Fraction(float(low))) / 15)

@@ -96,6 +96,16 @@ def test_pool_size(L):
     assert L.dc_kv4_pages_size(1, 8, 32, None) == 1
 
 
+def test_workspace_size_grows(L):
+    """A workspace of B sequences of D channels holds those of smaller calls."""
+    size = L.dc_aft_decode4_workspace_size
+    assert size(0, 64) == 0 and size(3, 40) == 0
+    last = 0
+    for D in range(32, 2100, 32):
+        assert size(64, D) >= last and size(63, D) <= size(64, D)
+        last = size(64, D)
+
+
 def test_python_calls_refuse_host_tensors():
     """The Python layer refuses tensors that are not on the current device
     before it reaches the library."""
