@@ -363,7 +363,7 @@ __device__ __forceinline__ float fmax_nan(float a, float b)
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 3;
 constexpr int kRows = 16;  // history rows of a block: two halves, each within a page
-constexpr int kStages = 3;  // blocks in flight of a warp
+constexpr int kStages = 2;  // blocks in flight of a warp
 constexpr int kItem = 10;   // what an item costs a CTA besides its blocks, in blocks
 
 // 16 bytes, of which the first `bytes` (0 or 16) are read, the others zeros
@@ -603,340 +603,340 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         const int blk = max(0, off - kItem), n = off + taken - kItem - blk;  // the share's blocks
         const int64_t u_item = u - off;
         if (n > 0) {
-        const int32_t *tab = p.table + b * p.ldtab;
-        const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + slab * W;
-        const float *w[NH];  // bias rows of this lane's octets
+            const int32_t *tab = p.table + b * p.ldtab;
+            const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + slab * W;
+            const float *w[NH];  // bias rows of this lane's octets
 #pragma unroll
-        for (int h = 0; h < NH; ++h)
-            w[h] = p.w + ((slab * W + group * 32 + (h ^ (2 * flip)) * 8 * (NH > 1)) / p.hs) * p.wh + t * p.ldw + rq;
-        // this warp's blocks: k0, k0 + step, ... < n, RPW neighbours at once
-        constexpr int kStep = kWarps * RPW;
-        const int k0 = warp * RPW + sub;
-        const int rounds = max(0, (n - warp * RPW + kStep - 1) / kStep);
-        uint8_t *pool = p.pages + (size_t)slab * p.page_size * kRec;
-        // pages of a block's halves, -1 behind t and past the share
-        auto pages_of = [&](int it) {
-            const int k = k0 + it * kStep, i0 = (blk + k) * kRows;
-            return make_int2(k < n ? tab[i0 >> p.shift] : -1, k < n && i0 + 8 <= t ? tab[(i0 + 8) >> p.shift] : -1);
-        };
-        auto there = [&](int page) { return (uint32_t)page < (uint32_t)p.n_pages; };
-        auto record_of = [&](int i, int page) {
-            return pool + (size_t)(uint32_t)page * p.page_bytes + (uint32_t)(i & (p.page_size - 1)) * kRec;
-        };
-        // a half without a page is filled with zeros
-        auto fetch = [&](int it, int2 page) {
-            const int i0 = (blk + k0 + it * kStep) * kRows;
-            const uint32_t dst = mine + (it % kStages) * kStageBytes;
-            const bool a = there(page.x), c = there(page.y);
-            const uint8_t *s0 = record_of(i0, a ? page.x : 0) + oct * 16, *s1 = record_of(i0 + 8, c ? page.y : 0) + oct * 16;
+            for (int h = 0; h < NH; ++h)
+                w[h] = p.w + ((slab * W + group * 32 + (h ^ (2 * flip)) * 8 * (NH > 1)) / p.hs) * p.wh + t * p.ldw + rq;
+            // this warp's blocks: k0, k0 + step, ... < n, RPW neighbours at once
+            constexpr int kStep = kWarps * RPW;
+            const int k0 = warp * RPW + sub;
+            const int rounds = max(0, (n - warp * RPW + kStep - 1) / kStep);
+            uint8_t *pool = p.pages + (size_t)slab * p.page_size * kRec;
+            // pages of a block's halves, -1 behind t and past the share
+            auto pages_of = [&](int it) {
+                const int k = k0 + it * kStep, i0 = (blk + k) * kRows;
+                return make_int2(k < n ? tab[i0 >> p.shift] : -1, k < n && i0 + 8 <= t ? tab[(i0 + 8) >> p.shift] : -1);
+            };
+            auto there = [&](int page) { return (uint32_t)page < (uint32_t)p.n_pages; };
+            auto record_of = [&](int i, int page) {
+                return pool + (size_t)(uint32_t)page * p.page_bytes + (uint32_t)(i & (p.page_size - 1)) * kRec;
+            };
+            // a half without a page is filled with zeros
+            auto fetch = [&](int it, int2 page) {
+                const int i0 = (blk + k0 + it * kStep) * kRows;
+                const uint32_t dst = mine + (it % kStages) * kStageBytes;
+                const bool a = there(page.x), c = there(page.y);
+                const uint8_t *s0 = record_of(i0, a ? page.x : 0) + oct * 16, *s1 = record_of(i0 + 8, c ? page.y : 0) + oct * 16;
 #pragma unroll
-            for (int k = 0; k < 5; ++k) cp_async16(dst + k * (LPR * 16), s0 + k * (LPR * 16), a ? 16 : 0);
+                for (int k = 0; k < 5; ++k) cp_async16(dst + k * (LPR * 16), s0 + k * (LPR * 16), a ? 16 : 0);
 #pragma unroll
-            for (int k = 0; k < 5; ++k) cp_async16(dst + (5 + k) * (LPR * 16), s1 + k * (LPR * 16), c ? 16 : 0);
-            cp_async_commit();
-        };
-        // biases of this lane's rows, -inf behind t and without a page
-        auto biases = [&](int it, int2 page, float4 (&x)[NH]) {
-            const int i0 = (blk + k0 + it * kStep) * kRows;
-            const int left = there(rq < 8 ? page.x : page.y) ? t - i0 - rq : -1;
+                for (int k = 0; k < 5; ++k) cp_async16(dst + (5 + k) * (LPR * 16), s1 + k * (LPR * 16), c ? 16 : 0);
+                cp_async_commit();
+            };
+            // biases of this lane's rows, -inf behind t and without a page
+            auto biases = [&](int it, int2 page, float4 (&x)[NH]) {
+                const int i0 = (blk + k0 + it * kStep) * kRows;
+                const int left = there(rq < 8 ? page.x : page.y) ? t - i0 - rq : -1;
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                const float *src = w[h] + i0;
-                if (p.w4 && left >= 3)
-                    x[h] = *reinterpret_cast<const float4 *>(src);
-                else
-                    x[h] = make_float4(left >= 0 ? src[0] : -INFINITY, left >= 1 ? src[1] : -INFINITY,
-                                       left >= 2 ? src[2] : -INFINITY, left >= 3 ? src[3] : -INFINITY);
+                for (int h = 0; h < NH; ++h) {
+                    const float *src = w[h] + i0;
+                    if (p.w4 && left >= 3)
+                        x[h] = *reinterpret_cast<const float4 *>(src);
+                    else
+                        x[h] = make_float4(left >= 0 ? src[0] : -INFINITY, left >= 1 ? src[1] : -INFINITY,
+                                           left >= 2 ? src[2] : -INFINITY, left >= 3 ? src[3] : -INFINITY);
+                }
+            };
+            // position t: the lanes of its block quantise it, 8 channels each
+            const int tail = nb - 1 - blk - k0;  // rounds * kStep on, if it is this warp's
+            const bool owner = tail >= 0 && tail % kStep == 0 && nb - 1 - blk < n;
+            float fresh[2][8];
+            int home = -1;
+            if (owner) {
+                load8(row + p.D + oct * 8, fresh[0]);
+                load8(row + 2 * p.D + oct * 8, fresh[1]);
+                home = tab[t >> p.shift];
             }
-        };
-        // position t: the lanes of its block quantise it, 8 channels each
-        const int tail = nb - 1 - blk - k0;  // rounds * kStep on, if it is this warp's
-        const bool owner = tail >= 0 && tail % kStep == 0 && nb - 1 - blk < n;
-        float fresh[2][8];
-        int home = -1;
-        if (owner) {
-            load8(row + p.D + oct * 8, fresh[0]);
-            load8(row + 2 * p.D + oct * 8, fresh[1]);
-            home = tab[t >> p.shift];
-        }
-        // pages of the blocks in flight, the next one's at hand early
-        int2 page[kStages];
+            // pages of the blocks in flight, the next one's at hand early
+            int2 page[kStages];
 #pragma unroll
-        for (int s = 0; s < kStages; ++s) page[s] = pages_of(s);
+            for (int s = 0; s < kStages; ++s) page[s] = pages_of(s);
 #pragma unroll
-        for (int s = 0; s < kStages - 1; ++s) fetch(s, page[s]);
-        float4 wn[NH];
-        biases(0, page[0], wn);
-        uint2 nc = make_uint2(0, 0), np = nc;  // its codes and parameters
-        if (owner && there(home)) {
-            float st, lo, c[8];
-            const uint32_t lanes = 0xfu << (lane & ~3);
-            nc.x = quantise8(fresh[0], st, lo, c, lanes);
-            np.x = pack_params(st, lo);
-            nc.y = quantise8(fresh[1], st, lo, c, lanes);
-            np.y = pack_params(st, lo);
-            uint8_t *rec = record_of(t, home);
-            *reinterpret_cast<uint2 *>(rec + oct * 8) = nc;
-            if (oct % 4 == 0) *reinterpret_cast<uint2 *>(rec + W + oct * 2) = np;
-        }
+            for (int s = 0; s < kStages - 1; ++s) fetch(s, page[s]);
+            float4 wn[NH];
+            biases(0, page[0], wn);
+            uint2 nc = make_uint2(0, 0), np = nc;  // its codes and parameters
+            if (owner && there(home)) {
+                float st, lo, c[8];
+                const uint32_t lanes = 0xfu << (lane & ~3);
+                nc.x = quantise8(fresh[0], st, lo, c, lanes);
+                np.x = pack_params(st, lo);
+                nc.y = quantise8(fresh[1], st, lo, c, lanes);
+                np.y = pack_params(st, lo);
+                uint8_t *rec = record_of(t, home);
+                *reinterpret_cast<uint2 *>(rec + oct * 8) = nc;
+                if (oct % 4 == 0) *reinterpret_cast<uint2 *>(rec + W + oct * 2) = np;
+            }
 
-        // octet o, pair j (factors)
-        f32x2 num[4][4], den[4][4];
-        float ref[NH];
-#pragma unroll
-        for (int o = 0; o < 4; ++o)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) num[o][j] = den[o][j] = 0;
-#pragma unroll
-        for (int h = 0; h < NH; ++h) ref[h] = -INFINITY;
-#pragma unroll 1
-        for (int it = 0; it < rounds; ++it) {
-            fetch(it + kStages - 1, page[kStages - 1]);
-            const int2 now = page[0];
-#pragma unroll
-            for (int s = 0; s < kStages - 1; ++s) page[s] = page[s + 1];
-            page[kStages - 1] = pages_of(it + kStages);
-            float4 wl[NH];
-#pragma unroll
-            for (int h = 0; h < NH; ++h) wl[h] = wn[h];
-            biases(it + 1, page[0], wn);
-            cp_async_wait<kStages - 1>();
-            __syncwarp();
-            uint8_t *stage = ring[warp][it % kStages] + sub * (kRows * kRec);
-            const int at = k0 + it * kStep < n ? t - (blk + k0 + it * kStep) * kRows : -1;
-            if (__any_sync(0xffffffffu, at < kRows || !there(now.x) || !there(now.y))) {
-                // position t itself, or a half without a page
-                if (at >= 0 && oct == 0 && (!there(now.x) || (at >= 8 && !there(now.y)))) atomicOr(p.status, DC_DEVERR_PAGE);
-                if (at >= 0 && at < kRows) {  // and nothing behind it
-                    for (int r = at; r < kRows; ++r) {
-                        *reinterpret_cast<uint2 *>(stage + r * kRec + oct * 8) = r > at ? make_uint2(0, 0) : nc;
-                        if (oct % 4 == 0)
-                            *reinterpret_cast<uint2 *>(stage + r * kRec + W + oct * 2) = r > at ? make_uint2(0, 0) : np;
-                    }
-                }
-                __syncwarp();
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint8_t *rec = stage + (rq + r) * kRec;
-                uint2 code[4];
-                if (kRec % 16 == 0) {
-                    const uint4 c = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 * flip);
-                    const uint4 d = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 - 16 * flip);
-                    code[0] = make_uint2(c.x, c.y);
-                    code[1] = make_uint2(c.z, c.w);
-                    code[2] = make_uint2(d.x, d.y);
-                    code[3] = make_uint2(d.z, d.w);
-                } else {
-#pragma unroll
-                    for (int o = 0; o < 4; ++o)
-                        code[o] = *reinterpret_cast<const uint2 *>(rec + group * 32 + (o ^ (2 * flip)) * 8);
-                }
-                const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + group * 8);
-                // value = low + step c = (low - 16 step) + 32 step (1/2 + c/32),
-                // exact in fp32 unless low outweighs step 2^15 times
-                const float kstep = __uint_as_float(par.x << 16), vstep = __uint_as_float(par.y << 16);
-                const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
-                const float va = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u)), vs = 32.f * vstep;
-                float ks[NH], ka[NH];  // y - ref = ka + ks (1/2 + c/32)
-#pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
-                    ks[h] = kstep * (32.f * kLog2e);
-                    ka[h] = fmaf(klow, kLog2e, x * kLog2e);
-                    if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
-                        // a finite bias of such size (a mask of -FLT_MAX)
-                        // absorbs the keys, in fp32 as in 64 bits
-                        ks[h] = 0.f;
-                        ka[h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
-                    }
-                    const float top = fmaf(ks[h], 31.f / 32.f, ka[h]);
-                    if (!(top <= ref[h] + 16.f)) {  // also where either is NaN
-                        const float scale = ex2(ref[h] - top);
-#pragma unroll
-                        for (int o = 0; o < 4; ++o)
-                            if (NH == 1 || o == h)
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    num[o][j] = mul2(num[o][j], pack2(scale, scale));
-                                    den[o][j] = mul2(den[o][j], pack2(scale, scale));
-                                }
-                        ref[h] = top;
-                    }
-                    if (ref[h] != -INFINITY) ka[h] -= ref[h];
-                }
-                f32x2 ks2[NH], ka2[NH];
-                const f32x2 vs2 = pack2(vs, vs), va2 = pack2(va, va);
-#pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    ks2[h] = pack2(ks[h], ks[h]);
-                    ka2[h] = pack2(ka[h], ka[h]);
-                }
-#pragma unroll
-                for (int o = 0; o < 4; ++o) {
-                    const int h = NH == 1 ? 0 : o;
-                    const uint32_t k0 = code[o].x << 3 & 0x78787878u, k1 = code[o].x >> 1 & 0x78787878u;
-                    const uint32_t v0 = code[o].y << 3 & 0x78787878u, v1 = code[o].y >> 1 & 0x78787878u;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 y = unpack2(fma2(factors(k0, k1, j), ks2[h], ka2[h]));
-                        const f32x2 e = pack2(ex2(y.x), ex2(y.y));
-                        const f32x2 v = fma2(factors(v0, v1, j), vs2, va2);
-                        num[o][j] = fma2(e, v, num[o][j]);
-                        den[o][j] = add2(den[o][j], e);
-                    }
-                }
-            }
-            __syncwarp();  // the stage may be filled again
-        }
-        cp_async_wait<0>();
-        __syncwarp();
-        // the lanes of a group: one ref, then sums over their NL lanes
-        constexpr int NL = 32 / NG;
-        float *sums = part(warp);  // [NL][2][W], then ref, num, den [3][W]
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-            float r = ref[h];
-#pragma unroll
-            for (int x = NG; x < 32; x *= 2) r = fmax_nan(r, __shfl_xor_sync(0xffffffffu, r, x));
-            const float scale = ref[h] == -INFINITY ? 0.f : ex2(ref[h] - r);
-            ref[h] = r;
+            // octet o, pair j (factors)
+            f32x2 num[4][4], den[4][4];
+            float ref[NH];
 #pragma unroll
             for (int o = 0; o < 4; ++o)
-                if (NH == 1 || o == h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        num[o][j] = mul2(num[o][j], pack2(scale, scale));
-                        den[o][j] = mul2(den[o][j], pack2(scale, scale));
+                for (int j = 0; j < 4; ++j) num[o][j] = den[o][j] = 0;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) ref[h] = -INFINITY;
+#pragma unroll 1
+            for (int it = 0; it < rounds; ++it) {
+                fetch(it + kStages - 1, page[kStages - 1]);
+                const int2 now = page[0];
+#pragma unroll
+                for (int s = 0; s < kStages - 1; ++s) page[s] = page[s + 1];
+                page[kStages - 1] = pages_of(it + kStages);
+                float4 wl[NH];
+#pragma unroll
+                for (int h = 0; h < NH; ++h) wl[h] = wn[h];
+                biases(it + 1, page[0], wn);
+                cp_async_wait<kStages - 1>();
+                __syncwarp();
+                uint8_t *stage = ring[warp][it % kStages] + sub * (kRows * kRec);
+                const int at = k0 + it * kStep < n ? t - (blk + k0 + it * kStep) * kRows : -1;
+                if (__any_sync(0xffffffffu, at < kRows || !there(now.x) || !there(now.y))) {
+                    // position t itself, or a half without a page
+                    if (at >= 0 && oct == 0 && (!there(now.x) || (at >= 8 && !there(now.y)))) atomicOr(p.status, DC_DEVERR_PAGE);
+                    if (at >= 0 && at < kRows) {  // and nothing behind it
+                        for (int r = at; r < kRows; ++r) {
+                            *reinterpret_cast<uint2 *>(stage + r * kRec + oct * 8) = r > at ? make_uint2(0, 0) : nc;
+                            if (oct % 4 == 0)
+                                *reinterpret_cast<uint2 *>(stage + r * kRec + W + oct * 2) = r > at ? make_uint2(0, 0) : np;
+                        }
                     }
-        }
+                    __syncwarp();
+                }
 #pragma unroll
-        for (int o = 0; o < 4; ++o) {
-            float *to = sums + (lane / NG) * 2 * W + group * 32 + (o ^ (2 * flip)) * 8;
-            float2 m[4], d[4];
+                for (int r = 0; r < 4; ++r) {
+                    const uint8_t *rec = stage + (rq + r) * kRec;
+                    uint2 code[4];
+                    if (kRec % 16 == 0) {
+                        const uint4 c = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 * flip);
+                        const uint4 d = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 - 16 * flip);
+                        code[0] = make_uint2(c.x, c.y);
+                        code[1] = make_uint2(c.z, c.w);
+                        code[2] = make_uint2(d.x, d.y);
+                        code[3] = make_uint2(d.z, d.w);
+                    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m[j] = unpack2(num[o][j]);
-                d[j] = unpack2(den[o][j]);
+                        for (int o = 0; o < 4; ++o)
+                            code[o] = *reinterpret_cast<const uint2 *>(rec + group * 32 + (o ^ (2 * flip)) * 8);
+                    }
+                    const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + group * 8);
+                    // value = low + step c = (low - 16 step) + 32 step (1/2 + c/32),
+                    // exact in fp32 unless low outweighs step 2^15 times
+                    const float kstep = __uint_as_float(par.x << 16), vstep = __uint_as_float(par.y << 16);
+                    const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
+                    const float va = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u)), vs = 32.f * vstep;
+                    float ks[NH], ka[NH];  // y - ref = ka + ks (1/2 + c/32)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) {
+                        const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
+                        ks[h] = kstep * (32.f * kLog2e);
+                        ka[h] = fmaf(klow, kLog2e, x * kLog2e);
+                        if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
+                            // a finite bias of such size (a mask of -FLT_MAX)
+                            // absorbs the keys, in fp32 as in 64 bits
+                            ks[h] = 0.f;
+                            ka[h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
+                        }
+                        const float top = fmaf(ks[h], 31.f / 32.f, ka[h]);
+                        if (!(top <= ref[h] + 16.f)) {  // also where either is NaN
+                            const float scale = ex2(ref[h] - top);
+#pragma unroll
+                            for (int o = 0; o < 4; ++o)
+                                if (NH == 1 || o == h)
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        num[o][j] = mul2(num[o][j], pack2(scale, scale));
+                                        den[o][j] = mul2(den[o][j], pack2(scale, scale));
+                                    }
+                            ref[h] = top;
+                        }
+                        if (ref[h] != -INFINITY) ka[h] -= ref[h];
+                    }
+                    f32x2 ks2[NH], ka2[NH];
+                    const f32x2 vs2 = pack2(vs, vs), va2 = pack2(va, va);
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) {
+                        ks2[h] = pack2(ks[h], ks[h]);
+                        ka2[h] = pack2(ka[h], ka[h]);
+                    }
+#pragma unroll
+                    for (int o = 0; o < 4; ++o) {
+                        const int h = NH == 1 ? 0 : o;
+                        const uint32_t k0 = code[o].x << 3 & 0x78787878u, k1 = code[o].x >> 1 & 0x78787878u;
+                        const uint32_t v0 = code[o].y << 3 & 0x78787878u, v1 = code[o].y >> 1 & 0x78787878u;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 y = unpack2(fma2(factors(k0, k1, j), ks2[h], ka2[h]));
+                            const f32x2 e = pack2(ex2(y.x), ex2(y.y));
+                            const f32x2 v = fma2(factors(v0, v1, j), vs2, va2);
+                            num[o][j] = fma2(e, v, num[o][j]);
+                            den[o][j] = add2(den[o][j], e);
+                        }
+                    }
+                }
+                __syncwarp();  // the stage may be filled again
             }
-            store8(to, {m[0].x, m[2].x, m[0].y, m[2].y, m[1].x, m[3].x, m[1].y, m[3].y});
-            store8(to + W, {d[0].x, d[2].x, d[0].y, d[2].y, d[1].x, d[3].x, d[1].y, d[3].y});
-        }
-        __syncwarp();
-        float sn[W / 32], sd[W / 32];
+            cp_async_wait<0>();
+            __syncwarp();
+            // the lanes of a group: one ref, then sums over their NL lanes
+            constexpr int NL = 32 / NG;
+            float *sums = part(warp);  // [NL][2][W], then ref, num, den [3][W]
 #pragma unroll
-        for (int k = 0; k < W / 32; ++k) {
-            sn[k] = sd[k] = 0.f;
+            for (int h = 0; h < NH; ++h) {
+                float r = ref[h];
+#pragma unroll
+                for (int x = NG; x < 32; x *= 2) r = fmax_nan(r, __shfl_xor_sync(0xffffffffu, r, x));
+                const float scale = ref[h] == -INFINITY ? 0.f : ex2(ref[h] - r);
+                ref[h] = r;
+#pragma unroll
+                for (int o = 0; o < 4; ++o)
+                    if (NH == 1 || o == h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            num[o][j] = mul2(num[o][j], pack2(scale, scale));
+                            den[o][j] = mul2(den[o][j], pack2(scale, scale));
+                        }
+            }
+#pragma unroll
+            for (int o = 0; o < 4; ++o) {
+                float *to = sums + (lane / NG) * 2 * W + group * 32 + (o ^ (2 * flip)) * 8;
+                float2 m[4], d[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    m[j] = unpack2(num[o][j]);
+                    d[j] = unpack2(den[o][j]);
+                }
+                store8(to, {m[0].x, m[2].x, m[0].y, m[2].y, m[1].x, m[3].x, m[1].y, m[3].y});
+                store8(to + W, {d[0].x, d[2].x, d[0].y, d[2].y, d[1].x, d[3].x, d[1].y, d[3].y});
+            }
+            __syncwarp();
+            float sn[W / 32], sd[W / 32];
+#pragma unroll
+            for (int k = 0; k < W / 32; ++k) {
+                sn[k] = sd[k] = 0.f;
 #pragma unroll (NL < 8 ? NL : 8)
-            for (int l = 0; l < NL; ++l) {
-                sn[k] += sums[l * 2 * W + k * 32 + lane];
-                sd[k] += sums[(l * 2 + 1) * W + k * 32 + lane];
+                for (int l = 0; l < NL; ++l) {
+                    sn[k] += sums[l * 2 * W + k * 32 + lane];
+                    sd[k] += sums[(l * 2 + 1) * W + k * 32 + lane];
+                }
             }
-        }
-        __syncwarp();
+            __syncwarp();
 #pragma unroll
-        for (int k = 0; k < W / 32; ++k) {
-            sums[W + k * 32 + lane] = sn[k];
-            sums[2 * W + k * 32 + lane] = sd[k];
-        }
-#pragma unroll
-        for (int o = 0; o < 4; ++o)
-            if (lane / NG == o) {
-                const float r = ref[o % NH];
-                store8(sums + group * 32 + (o ^ (2 * flip)) * 8, {r, r, r, r, r, r, r, r});
+            for (int k = 0; k < W / 32; ++k) {
+                sums[W + k * 32 + lane] = sn[k];
+                sums[2 * W + k * 32 + lane] = sd[k];
             }
-        __syncthreads();
-        constexpr int CPT = (W + kThreads - 1) / kThreads;  // channels a thread finishes
-        float fm[CPT], fn[CPT], fd[CPT];
 #pragma unroll
-        for (int k = 0; k < CPT; ++k) {
-            const int c = tid + k * kThreads;
-            if (c >= W) continue;
-            fm[k] = part(0)[c];
-            fn[k] = part(0)[W + c];
-            fd[k] = part(0)[2 * W + c];
-#pragma unroll
-            for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part(g)[c], part(g)[W + c], part(g)[2 * W + c]);
-        }
-        bool finish = n == nb;
-        if (!finish) {  // shared with other CTAs
-            // second slot: an item that begins inside the CTA's share
-            const auto slot = [&](int g) { return (int64_t)g * 2 + (!even && u_item > (int64_t)g * q); };
-            float *mine = p.part + slot(blockIdx.x) * 3 * W;
+            for (int o = 0; o < 4; ++o)
+                if (lane / NG == o) {
+                    const float r = ref[o % NH];
+                    store8(sums + group * 32 + (o ^ (2 * flip)) * 8, {r, r, r, r, r, r, r, r});
+                }
+            __syncthreads();
+            constexpr int CPT = (W + kThreads - 1) / kThreads;  // channels a thread finishes
+            float fm[CPT], fn[CPT], fd[CPT];
 #pragma unroll
             for (int k = 0; k < CPT; ++k) {
                 const int c = tid + k * kThreads;
                 if (c >= W) continue;
-                mine[c] = fm[k];
-                mine[W + c] = fn[k];
-                mine[2 * W + c] = fd[k];
+                fm[k] = part(0)[c];
+                fn[k] = part(0)[W + c];
+                fd[k] = part(0)[2 * W + c];
+#pragma unroll
+                for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part(g)[c], part(g)[W + c], part(g)[2 * W + c]);
             }
-            __threadfence();
-            __syncthreads();
-            if (!even) {
-                j0 = (int)((u_item + kItem) / q);
-                j1 = (int)((u_item + kItem + nb - 1) / q);
-            }
-            if (tid == 0) {
-                int *counter = p.counter + (int64_t)b * p.nslab + slab;
-                s_last = atomicAdd(counter, 1) == j1 - j0;
-                if (s_last) *counter = 0;  // ready for the next launch
-            }
-            __syncthreads();
-            if (s_last) {
-                finish = true;
-                __threadfence();
-#pragma unroll
-                for (int k = 0; k < CPT; ++k) {
-                    fm[k] = -INFINITY;
-                    fn[k] = fd[k] = 0.f;
-                }
-                constexpr int kAhead = 8;  // shares whose sums are read at once
-                for (int g0 = j0; g0 <= j1; g0 += kAhead) {
-                    float x[kAhead][CPT][3];
-#pragma unroll
-                    for (int d = 0; d < kAhead; ++d) {
-                        const float *src = p.part + slot(min(g0 + d, j1)) * 3 * W;
-#pragma unroll
-                        for (int k = 0; k < CPT; ++k) {
-                            const int c = min(tid + k * kThreads, W - 1);
-                            x[d][k][0] = __ldcg(src + c);
-                            x[d][k][1] = __ldcg(src + W + c);
-                            x[d][k][2] = __ldcg(src + 2 * W + c);
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < kAhead; ++d)
-#pragma unroll
-                        for (int k = 0; k < CPT; ++k)
-                            if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][k][0], x[d][k][1], x[d][k][2]);
-                }
-            }
-        }
-        if (finish) {
-            int lost = 0;
-#pragma unroll
-            for (int k = 0; k < CPT; ++k)
-                if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-90f) lost = 1;
-            if (__syncthreads_or(lost)) {
-                resum<W>(p, b, slab, t, part(0));
+            bool finish = n == nb;
+            if (!finish) {  // shared with other CTAs
+                // second slot: an item that begins inside the CTA's share
+                const auto slot = [&](int g) { return (int64_t)g * 2 + (!even && u_item > (int64_t)g * q); };
+                float *mine = p.part + slot(blockIdx.x) * 3 * W;
 #pragma unroll
                 for (int k = 0; k < CPT; ++k) {
                     const int c = tid + k * kThreads;
                     if (c >= W) continue;
-                    fn[k] = part(0)[c];
-                    fd[k] = part(0)[W + c];
+                    mine[c] = fm[k];
+                    mine[W + c] = fn[k];
+                    mine[2 * W + c] = fd[k];
+                }
+                __threadfence();
+                __syncthreads();
+                if (!even) {
+                    j0 = (int)((u_item + kItem) / q);
+                    j1 = (int)((u_item + kItem + nb - 1) / q);
+                }
+                if (tid == 0) {
+                    int *counter = p.counter + (int64_t)b * p.nslab + slab;
+                    s_last = atomicAdd(counter, 1) == j1 - j0;
+                    if (s_last) *counter = 0;  // ready for the next launch
+                }
+                __syncthreads();
+                if (s_last) {
+                    finish = true;
+                    __threadfence();
+#pragma unroll
+                    for (int k = 0; k < CPT; ++k) {
+                        fm[k] = -INFINITY;
+                        fn[k] = fd[k] = 0.f;
+                    }
+                    constexpr int kAhead = 8;  // shares whose sums are read at once
+                    for (int g0 = j0; g0 <= j1; g0 += kAhead) {
+                        float x[kAhead][CPT][3];
+#pragma unroll
+                        for (int d = 0; d < kAhead; ++d) {
+                            const float *src = p.part + slot(min(g0 + d, j1)) * 3 * W;
+#pragma unroll
+                            for (int k = 0; k < CPT; ++k) {
+                                const int c = min(tid + k * kThreads, W - 1);
+                                x[d][k][0] = __ldcg(src + c);
+                                x[d][k][1] = __ldcg(src + W + c);
+                                x[d][k][2] = __ldcg(src + 2 * W + c);
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < kAhead; ++d)
+#pragma unroll
+                            for (int k = 0; k < CPT; ++k)
+                                if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][k][0], x[d][k][1], x[d][k][2]);
+                    }
                 }
             }
+            if (finish) {
+                int lost = 0;
 #pragma unroll
-            for (int k = 0; k < CPT; ++k) {
-                const int c = tid + k * kThreads;
-                if (c >= W) continue;
-                const float qv = to_f<T>(row[c]);
-                static_cast<T *>(p.Z)[b * p.ldz + slab * W + c] =
-                    from_f<T>(fd[k] == 0.f ? 0.f : sigm(qv) * (fn[k] / fd[k]));
+                for (int k = 0; k < CPT; ++k)
+                    if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-90f) lost = 1;
+                if (__syncthreads_or(lost)) {
+                    resum<W>(p, b, slab, t, part(0));
+#pragma unroll
+                    for (int k = 0; k < CPT; ++k) {
+                        const int c = tid + k * kThreads;
+                        if (c >= W) continue;
+                        fn[k] = part(0)[c];
+                        fd[k] = part(0)[W + c];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < CPT; ++k) {
+                    const int c = tid + k * kThreads;
+                    if (c >= W) continue;
+                    const float qv = to_f<T>(row[c]);
+                    static_cast<T *>(p.Z)[b * p.ldz + slab * W + c] =
+                        from_f<T>(fd[k] == 0.f ? 0.f : sigm(qv) * (fn[k] / fd[k]));
+                }
             }
-        }
         }
         u += taken;
         if (u >= u1) return;
