@@ -221,9 +221,11 @@ __device__ __forceinline__ uint32_t quantise8(float (&x)[8], float &step, float 
         const f32x2 st2 = pack2(st, st);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const f32x2 border = add2(pack2(c[2 * j], c[2 * j + 1]), pack2(copysignf(0.5f, r[j].x), copysignf(0.5f, r[j].y)));
+            const f32x2 half = pack2(copysignf(0.5f, r[j].x), copysignf(0.5f, r[j].y));
+            const f32x2 border = add2(pack2(c[2 * j], c[2 * j + 1]), half);
             const float2 y = unpack2(fma2_ru(st2, border, lo2));
-            const float2 k = unpack2(add2(border, pack2(x[2 * j] >= y.x ? 0.5f : -0.5f, x[2 * j + 1] >= y.y ? 0.5f : -0.5f)));
+            const f32x2 side = pack2(x[2 * j] >= y.x ? 0.5f : -0.5f, x[2 * j + 1] >= y.y ? 0.5f : -0.5f);
+            const float2 k = unpack2(add2(border, side));
             c[2 * j] = k.x;
             c[2 * j + 1] = k.y;
         }
@@ -281,7 +283,11 @@ constexpr int kWriteWarps = 8;
 
 // A lane per 8 channels of a row (k and v), `span` lanes a row: a warp takes
 // 256 channels of a row (blockIdx.y which of them), or 32/span rows of fewer.
-// Rows with a negative slot are left out.  HBM-bound.
+// Rows with a negative slot are left out.  Bound by HBM and issue alike: 65521
+// rows of 2048 bf16 channels with their values back, 1.24 GB, take 270 us
+// (0.71 of the measured copy rate), about 25 instructions a value, a fifth of
+// them for borders, which bf16 values meet often; with a division for the
+// step and one a value it took 702 us.
 template <typename T>
 __global__ void __launch_bounds__(32 * kWriteWarps) write_kernel(const __grid_constant__ Write p, int span)
 {
@@ -473,7 +479,7 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 // (the group's largest value is low + 15 step) passes it by more than 16.
 //
 // A channel that lies so far below its group that its den is below 2^-90 has
-// lost terms to underflow: its share is then summed again with a running
+// lost terms to underflow: its item is then summed again with a running
 // maximum per channel.
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
@@ -482,6 +488,17 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 // costs little, each item into parts of its own, so that a CTA has one.  An
 // item that several CTAs share is merged, in CTA order, by the last of them
 // to finish.
+//
+// What bounds it: a channel of a position costs one 2^x (8 cycles a warp and
+// scheduler) and about 7 other instructions that overlap with it imperfectly
+// (9.5 cycles alone), against 1.25 bytes of HBM, so 32 sequences of up to 8191
+// positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 113 us; the
+// rest is what an item costs besides (merging, its first loads).  At 64
+// sequences of 256-511 positions, d = 512, these are most of the 16 us.  Steps
+// there: a lane per 8 channels 146 us (10.5 instructions a channel for
+// unpacking and bounds), 16 channels 183 us (too few registers), a group of 32
+// by four rows 141 us; codes through mixed-precision bf16 FMAs instead of byte
+// permutations were as fast, four CTAs an SM (128 registers) 20% slower.
 template <typename T, int W, int NH>
 __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __grid_constant__ Decode p)
 {
@@ -716,43 +733,43 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                     }
                     __syncwarp();
                 }
+                // rows whose exponents are bounded together: fewer branches between
+                // the sums (two with one bias a row: 116.6 -> 113 us; else one, for registers)
+                constexpr int kTogether = NH == 1 ? 2 : 1;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint8_t *rec = stage + (rq + r) * kRec;
-                    uint2 code[4];
-                    if (kRec % 16 == 0) {
-                        const uint4 c = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 * flip);
-                        const uint4 d = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 - 16 * flip);
-                        code[0] = make_uint2(c.x, c.y);
-                        code[1] = make_uint2(c.z, c.w);
-                        code[2] = make_uint2(d.x, d.y);
-                        code[3] = make_uint2(d.z, d.w);
-                    } else {
-#pragma unroll
-                        for (int o = 0; o < 4; ++o)
-                            code[o] = *reinterpret_cast<const uint2 *>(rec + group * 32 + (o ^ (2 * flip)) * 8);
-                    }
-                    const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + group * 8);
+                for (int r0 = 0; r0 < 4; r0 += kTogether) {
+                    // y - ref = ka + ks (1/2 + c/32), v = va + vs (1/2 + c/32):
                     // value = low + step c = (low - 16 step) + 32 step (1/2 + c/32),
                     // exact in fp32 unless low outweighs step 2^15 times
-                    const float kstep = __uint_as_float(par.x << 16), vstep = __uint_as_float(par.y << 16);
-                    const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
-                    const float va = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u)), vs = 32.f * vstep;
-                    float ks[NH], ka[NH];  // y - ref = ka + ks (1/2 + c/32)
+                    float ks[kTogether][NH], ka[kTogether][NH], vs[kTogether], va[kTogether], top[NH];
+#pragma unroll
+                    for (int h = 0; h < NH; ++h) top[h] = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kTogether; ++i) {
+                        const int r = r0 + i;
+                        const uint2 par = *reinterpret_cast<const uint2 *>(stage + (rq + r) * kRec + W + group * 8);
+                        const float kstep = __uint_as_float(par.x << 16), vstep = __uint_as_float(par.y << 16);
+                        const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
+                        va[i] = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u));
+                        vs[i] = 32.f * vstep;
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) {
+                            const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
+                            ks[i][h] = kstep * (32.f * kLog2e);
+                            ka[i][h] = fmaf(klow, kLog2e, x * kLog2e);
+                            if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
+                                // a finite bias of such size (a mask of -FLT_MAX)
+                                // absorbs the keys, in fp32 as in 64 bits
+                                ks[i][h] = 0.f;
+                                ka[i][h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
+                            }
+                            top[h] = fmax_nan(top[h], fmaf(ks[i][h], 31.f / 32.f, ka[i][h]));
+                        }
+                    }
 #pragma unroll
                     for (int h = 0; h < NH; ++h) {
-                        const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
-                        ks[h] = kstep * (32.f * kLog2e);
-                        ka[h] = fmaf(klow, kLog2e, x * kLog2e);
-                        if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
-                            // a finite bias of such size (a mask of -FLT_MAX)
-                            // absorbs the keys, in fp32 as in 64 bits
-                            ks[h] = 0.f;
-                            ka[h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
-                        }
-                        const float top = fmaf(ks[h], 31.f / 32.f, ka[h]);
-                        if (!(top <= ref[h] + 16.f)) {  // also where either is NaN
-                            const float scale = ex2(ref[h] - top);
+                        if (!(top[h] <= ref[h] + 16.f)) {  // also where either is NaN
+                            const float scale = ex2(ref[h] - top[h]);
 #pragma unroll
                             for (int o = 0; o < 4; ++o)
                                 if (NH == 1 || o == h)
@@ -761,29 +778,48 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                                         num[o][j] = mul2(num[o][j], pack2(scale, scale));
                                         den[o][j] = mul2(den[o][j], pack2(scale, scale));
                                     }
-                            ref[h] = top;
+                            ref[h] = top[h];
                         }
-                        if (ref[h] != -INFINITY) ka[h] -= ref[h];
-                    }
-                    f32x2 ks2[NH], ka2[NH];
-                    const f32x2 vs2 = pack2(vs, vs), va2 = pack2(va, va);
+                        const float base = ref[h] == -INFINITY ? 0.f : ref[h];
 #pragma unroll
-                    for (int h = 0; h < NH; ++h) {
-                        ks2[h] = pack2(ks[h], ks[h]);
-                        ka2[h] = pack2(ka[h], ka[h]);
+                        for (int i = 0; i < kTogether; ++i) ka[i][h] -= base;
                     }
 #pragma unroll
-                    for (int o = 0; o < 4; ++o) {
-                        const int h = NH == 1 ? 0 : o;
-                        const uint32_t k0 = code[o].x << 3 & 0x78787878u, k1 = code[o].x >> 1 & 0x78787878u;
-                        const uint32_t v0 = code[o].y << 3 & 0x78787878u, v1 = code[o].y >> 1 & 0x78787878u;
+                    for (int i = 0; i < kTogether; ++i) {
+                        const uint8_t *rec = stage + (rq + r0 + i) * kRec;
+                        uint2 code[4];
+                        if (kRec % 16 == 0) {
+                            const uint4 c = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 * flip);
+                            const uint4 d = *reinterpret_cast<const uint4 *>(rec + group * 32 + 16 - 16 * flip);
+                            code[0] = make_uint2(c.x, c.y);
+                            code[1] = make_uint2(c.z, c.w);
+                            code[2] = make_uint2(d.x, d.y);
+                            code[3] = make_uint2(d.z, d.w);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 y = unpack2(fma2(factors(k0, k1, j), ks2[h], ka2[h]));
-                            const f32x2 e = pack2(ex2(y.x), ex2(y.y));
-                            const f32x2 v = fma2(factors(v0, v1, j), vs2, va2);
-                            num[o][j] = fma2(e, v, num[o][j]);
-                            den[o][j] = add2(den[o][j], e);
+                            for (int o = 0; o < 4; ++o)
+                                code[o] = *reinterpret_cast<const uint2 *>(rec + group * 32 + (o ^ (2 * flip)) * 8);
+                        }
+                        f32x2 ks2[NH], ka2[NH];
+                        const f32x2 vs2 = pack2(vs[i], vs[i]), va2 = pack2(va[i], va[i]);
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) {
+                            ks2[h] = pack2(ks[i][h], ks[i][h]);
+                            ka2[h] = pack2(ka[i][h], ka[i][h]);
+                        }
+#pragma unroll
+                        for (int o = 0; o < 4; ++o) {
+                            const int h = NH == 1 ? 0 : o;
+                            const uint32_t k0 = code[o].x << 3 & 0x78787878u, k1 = code[o].x >> 1 & 0x78787878u;
+                            const uint32_t v0 = code[o].y << 3 & 0x78787878u, v1 = code[o].y >> 1 & 0x78787878u;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float2 y = unpack2(fma2(factors(k0, k1, j), ks2[h], ka2[h]));
+                                const f32x2 e = pack2(ex2(y.x), ex2(y.y));
+                                const f32x2 v = fma2(factors(v0, v1, j), vs2, va2);
+                                num[o][j] = fma2(e, v, num[o][j]);
+                                den[o][j] = add2(den[o][j], e);
+                            }
                         }
                     }
                 }
