@@ -279,17 +279,17 @@ struct Write {
     int *status;
 };
 
-constexpr int kWriteWarps = 8;
+constexpr int kWriteWarps = 4;
 
 // A lane per 8 channels of a row (k and v), `span` lanes a row: a warp takes
 // 256 channels of a row (blockIdx.y which of them), or 32/span rows of fewer.
 // Rows with a negative slot are left out.  Bound by HBM and issue alike: 65521
-// rows of 2048 bf16 channels with their values back, 1.24 GB, take 270 us
-// (0.71 of the measured copy rate), about 25 instructions a value, a fifth of
+// rows of 2048 bf16 channels with their values back, 1.24 GB, take 264 us
+// (0.73 of the measured copy rate), about 25 instructions a value, a fifth of
 // them for borders, which bf16 values meet often; with a division for the
 // step and one a value it took 702 us.
 template <typename T>
-__global__ void __launch_bounds__(32 * kWriteWarps) write_kernel(const __grid_constant__ Write p, int span)
+__global__ void __launch_bounds__(32 * kWriteWarps, 9) write_kernel(const __grid_constant__ Write p, int span)
 {
     grid_dep_wait();  // programmatic dependent launch: inputs are ready
     grid_dep_launch();
@@ -462,7 +462,10 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
     __syncthreads();
     for (int c = threadIdx.x; c < W; c += kThreads) {
         float mc = out[2 * W + c], nc = out[c], dc = out[W + c];
-        for (int g = 1; g < kWarps; ++g) add(mc, nc, dc, out[(g * 3 + 2) * W + c], out[g * 3 * W + c], out[(g * 3 + 1) * W + c]);
+        for (int g = 1; g < kWarps; ++g) {
+            const float *src = out + g * 3 * W + c;
+            add(mc, nc, dc, src[2 * W], src[0], src[W]);
+        }
         out[c] = nc;
         out[W + c] = dc;
     }
@@ -552,6 +555,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         active += s_active[k];
     }
     const int64_t total = (int64_t)sum * p.nslab, items = (int64_t)active * p.nslab;
+    if (items == 0) return;
     const int64_t units = total + items * kItem;
     const int G = gridDim.x;
     // at least some rounds of the CTA's warps, so that merging a long sequence's
@@ -564,8 +568,20 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     int64_t even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), (int64_t)least) : INT32_MAX;
     const bool even = even_q <= q + 6;
     if (even) q = (int)even_q;
+    const int fewer = (q - 1) / (kWarps * RPW) * (kWarps * RPW);
+    if (even && p.B <= kThreads && fewer >= max(1, least)) {
+        // parts of one round of the warps less, where rounding leaves the CTAs
+        const int parts = __reduce_add_sync(0xffffffffu, (nb + fewer - 1) / fewer);
+        __syncthreads();
+        if (lane == 0) s_sum[warp] = parts;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) all += s_sum[k];
+        if ((int64_t)all * p.nslab <= G) q = fewer;
+    }
     auto weight = [&](int nb) {  // CTAs, or blocks and what an item costs besides
-        return even ? (nb + q - 1) / q : nb ? nb + kItem : 0;
+        return nb == 0 ? 0 : even ? (nb + q - 1) / q : nb + kItem;
     };
     // this CTA's share: [u, u1) of all slabs' weights, one sequence after the other
     int64_t u = even ? blockIdx.x : (int64_t)blockIdx.x * q;
@@ -645,7 +661,8 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 const int i0 = (blk + k0 + it * kStep) * kRows;
                 const uint32_t dst = mine + (it % kStages) * kStageBytes;
                 const bool a = there(page.x), c = there(page.y);
-                const uint8_t *s0 = record_of(i0, a ? page.x : 0) + oct * 16, *s1 = record_of(i0 + 8, c ? page.y : 0) + oct * 16;
+                const uint8_t *s0 = record_of(i0, a ? page.x : 0) + oct * 16;
+                const uint8_t *s1 = record_of(i0 + 8, c ? page.y : 0) + oct * 16;
 #pragma unroll
                 for (int k = 0; k < 5; ++k) cp_async16(dst + k * (LPR * 16), s0 + k * (LPR * 16), a ? 16 : 0);
 #pragma unroll
@@ -723,12 +740,14 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 const int at = k0 + it * kStep < n ? t - (blk + k0 + it * kStep) * kRows : -1;
                 if (__any_sync(0xffffffffu, at < kRows || !there(now.x) || !there(now.y))) {
                     // position t itself, or a half without a page
-                    if (at >= 0 && oct == 0 && (!there(now.x) || (at >= 8 && !there(now.y)))) atomicOr(p.status, DC_DEVERR_PAGE);
+                    if (at >= 0 && oct == 0 && (!there(now.x) || (at >= 8 && !there(now.y))))
+                        atomicOr(p.status, DC_DEVERR_PAGE);
                     if (at >= 0 && at < kRows) {  // and nothing behind it
                         for (int r = at; r < kRows; ++r) {
-                            *reinterpret_cast<uint2 *>(stage + r * kRec + oct * 8) = r > at ? make_uint2(0, 0) : nc;
+                            uint8_t *to = stage + r * kRec;
+                            *reinterpret_cast<uint2 *>(to + oct * 8) = r > at ? make_uint2(0, 0) : nc;
                             if (oct % 4 == 0)
-                                *reinterpret_cast<uint2 *>(stage + r * kRec + W + oct * 2) = r > at ? make_uint2(0, 0) : np;
+                                *reinterpret_cast<uint2 *>(to + W + oct * 2) = r > at ? make_uint2(0, 0) : np;
                         }
                     }
                     __syncwarp();
@@ -892,7 +911,8 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 fn[k] = part(0)[W + c];
                 fd[k] = part(0)[2 * W + c];
 #pragma unroll
-                for (int g = 1; g < kWarps; ++g) join(fm[k], fn[k], fd[k], part(g)[c], part(g)[W + c], part(g)[2 * W + c]);
+                for (int g = 1; g < kWarps; ++g)
+                    join(fm[k], fn[k], fd[k], part(g)[c], part(g)[W + c], part(g)[2 * W + c]);
             }
             bool finish = n == nb;
             if (!finish) {  // shared with other CTAs
@@ -1085,7 +1105,8 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
     int span = 4;  // lanes a row
     while (span < 32 && span * 8 < D) span *= 2;
     const int chunks = (D + 255) / 256, rows = kWriteWarps * (32 / span);
-    const dim3 grid(std::min((n - 1) / rows + 1, std::max(1, sm_count() * 32 / chunks)), chunks), block(32 * kWriteWarps);
+    const int most = std::max(1, sm_count() * 64 / chunks);
+    const dim3 grid(std::min((n - 1) / rows + 1, most), chunks), block(32 * kWriteWarps);
     DC_CUDA_TRY(dtype == DC_F32 ? launch_pdl(write_kernel<float>, grid, block, 0, st, 1, p, span)
                                 : launch_pdl(write_kernel<__nv_bfloat16>, grid, block, 0, st, 1, p, span));
     return DC_OK;

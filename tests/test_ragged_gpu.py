@@ -522,7 +522,7 @@ def test_logits_controls(ops, B, V, T, dtype, which, ld):
     # then one rounding to the type
     size = 1.6 * np.abs(host[:, :V].float().numpy()).max() + 0.6 * T + 1 + 5
     tol = 5 * 2.0**-24 * size + (2.0**-8 if dtype == "bf16" else 0) * np.abs(np.where(ok, want, 0))
-    assert np.all(np.abs(np.where(ok, g - want, 0)) <= tol)
+    assert np.all(np.abs(np.where(ok, g, 0) - np.where(ok, want, 0)) <= tol)
     # in place
     y = host.cuda()
     ops.logits_controls(y[:, :V], cu(tokens), cu(pos), prompt_len=cu(prompt), repetition=opt(rep), presence=opt(pres),
