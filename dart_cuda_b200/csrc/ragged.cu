@@ -521,15 +521,16 @@ int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_s
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("page_tables", st);
     p.slots4 = aligned16(slots);
-    // One CTA for a decode step or a few prompts (3.6 us for 64 requests of
-    // one token; 148 CTAs 4.5 us); for more tokens a CTA per 4096 slots, or
-    // per 32 requests of new pages, up to one an SM (500 prompts of 1024
-    // tokens: 504 us on one CTA).
-    const int64_t work = std::max<int64_t>(slots ? n_slots : 0, (int64_t)128 * B);
-    const int grid = B <= kTabThreads && (slots ? n_slots : 0) <= 8192
-                         ? 1 : (int)std::min<int64_t>(sm_count(), (work + 4095) / 4096);
+    // A CTA per 1024 slots, or per 16 requests, up to one an SM (64 prompts of
+    // 127 tokens: 5.0 us, per 4096 slots 6.2, on one CTA 6.8; 500 prompts of 1024
+    // tokens: 6.4 us, on one CTA 504).  A head that is advanced in place takes
+    // two launches then, and one CTA while that is faster.
+    const int64_t room = slots ? n_slots : 0, work = std::max<int64_t>(room, (int64_t)64 * B);
+    const bool in_place = free_head == free_head_out;
+    const int grid = in_place && B <= kTabThreads && room <= 8192
+                         ? 1 : (int)std::min<int64_t>(sm_count(), (work + 1023) / 1024);
     int last = grid;
-    if (grid > 1 && free_head == free_head_out) {
+    if (grid > 1 && in_place) {
         // other CTAs may still have to read the head that one would advance:
         // a second launch of one CTA does (and writes the same entries again)
         p.head_out = nullptr;
@@ -568,9 +569,9 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
     p.ldo = ldo;
     p.B = B;
     p.V = V;
-    // chunks of 1024 while the grid is short of four blocks an SM, of at most
-    // 16384 (64 KB of counts)
-    const int64_t fill = (4LL * sm_count() + B - 1) / B;
+    // chunks of 1024 while the grid is short of eight blocks an SM (64 x 32000
+    // fp32: 6.3 us, four 7.4, twelve 7.2), of at most 16384 (64 KB of counts)
+    const int64_t fill = (8LL * sm_count() + B - 1) / B;
     const int64_t want = std::max<int64_t>((V + 16383) / 16384, std::min<int64_t>((V + 1023) / 1024, fill));
     p.chunk = (int)round_up((V + want - 1) / want, 32);
     p.chunks = (V + p.chunk - 1) / p.chunk;
@@ -589,7 +590,10 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
     if ((int64_t)B * p.chunks > INT32_MAX) return fail(DC_ERR_INVALID, "B * V too large");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("logits_controls", st);
-    const dim3 grid((unsigned)(B * p.chunks)), block(p.chunk > 4096 ? 512 : 256);
+    // long chunks leave room for few blocks an SM: more threads in each (64 x
+    // 50257 in chunks of 2656: 256 threads 8.1 us, 512 10.4; 512 x 50257 in
+    // chunks of 12576, one bias and mask: 512 threads 40 us, 256 50)
+    const dim3 grid((unsigned)(B * p.chunks)), block(p.chunk > 8192 ? 512 : 256);
     const int smem = pens ? p.chunk * (int)sizeof(uint32_t) : 0;
     auto kernel = dtype == DC_F32 ? logits_kernel<float> : logits_kernel<__nv_bfloat16>;
     if (smem > 48 * 1024) {
@@ -627,10 +631,17 @@ int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, c
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("greedy_embed_rows", st);
-    // a cluster a row while rows are few and long (one row of 131072 logits:
-    // 8 blocks against 1)
-    p.cluster = V >= 16384 && B <= sm_count() / 4 ? 8 : 1;
-    const dim3 grid((unsigned)(B * p.cluster)), block(V > 2048 ? 512 : 128);
+    // A cluster of 4 blocks a row while rows are few and long: rows of 131072
+    // fp32 logits take 5.8 us instead of 9.1 (1 row), 9.7 instead of 16.2 (64);
+    // at 32768 logits one block is as fast or faster (4.3 us both, against 4.4
+    // and 5.3).
+    // 8 blocks gain up to 1 us on one row and lose 3 us on 37.
+    p.cluster = V >= 65536 && B <= sm_count() / 2 ? 4 : 1;
+    // Fewer threads for short rows (64 x 2048: 256 threads 2.5 us, 512 2.65) and
+    // for so many that blocks queue (512 x 512: 128 threads 3.0 us, 256 3.2, 512
+    // 4.7; 512 x 8192: 256 threads 4.8 us, 512 6.2; 64 x 8192: 3.0 and 2.8).
+    const int threads = 512 >> (V <= 2048) >> (V <= 16384 && B > 2 * sm_count());
+    const dim3 grid((unsigned)(B * p.cluster)), block(threads);
     auto kernel = dtype == DC_F32 ? pick_kernel<float> : pick_kernel<__nv_bfloat16>;
     DC_CUDA_TRY(launch_pdl(kernel, grid, block, 0, st, p.cluster, p));
     return DC_OK;

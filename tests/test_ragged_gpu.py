@@ -293,6 +293,16 @@ def test_aft_decode4_long(ops, H, hs, T, page, dtype, lens):
     History(ops, rng, len(lens), H, hs, T, page, dtype, lens).check()
 
 
+@pytest.mark.parametrize("masked", [0, 4800])
+def test_aft_decode4_many_shares(ops, masked):
+    """One sequence over many CTAs, whose first shares a mask may leave empty."""
+    T = 5000
+    rng = np.random.default_rng(masked)
+    w = (0.5 * rng.standard_normal((1, T, T))).astype(np.float32)
+    w[:, :, :masked] = -np.inf
+    History(ops, rng, 2, 1, 64, T, 32, "f32", [T - 1, T - 100], w=w).check()
+
+
 def test_aft_decode4_many_sequences(ops):
     """More sequences than SMs, lengths from one to long, in one call."""
     rng = np.random.default_rng(3)
@@ -565,7 +575,8 @@ def test_logits_controls_long_history(ops):
 
 # ------------------------------------------------------------ pick
 @pytest.mark.parametrize("B,V,D,dtype,ld", [(1, 1, 1, "f32", 0), (3, 65, 32, "f32", 0), (64, 8192, 512, "f32", 0),
-                                            (5, 50257, 48, "bf16", 3), (2, 131073, 7, "f32", 1), (300, 130, 4, "bf16", 0)])
+                                            (5, 50257, 48, "bf16", 3), (2, 131073, 7, "f32", 1), (300, 130, 4, "bf16", 0),
+                                            (40, 70001, 9, "bf16", 3), (400, 9000, 5, "f32", 1)])
 def test_greedy_embed_rows(ops, B, V, D, dtype, ld):
     rng = np.random.default_rng(V)
     T = 12
