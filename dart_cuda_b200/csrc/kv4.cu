@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "dc_internal.h"
 #include "dc_ptx.cuh"
@@ -497,7 +498,7 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 // (9.5 cycles alone), against 1.25 bytes of HBM, so 32 sequences of up to 8191
 // positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 113 us; the
 // rest is what an item costs besides (merging, its first loads).  At 64
-// sequences of 256-511 positions, d = 512, these are most of the 16 us.  Steps
+// sequences of 256-511 positions, d = 512, these are most of the 15 us.  Steps
 // there: a lane per 8 channels 146 us (10.5 instructions a channel for
 // unpacking and bounds), 16 channels 183 us (too few registers), a group of 32
 // by four rows 141 us; codes through mixed-precision bf16 FMAs instead of byte
@@ -559,18 +560,21 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     const int64_t units = total + items * kItem;
     const int G = gridDim.x;
     // at least some rounds of the CTA's warps, so that merging a long sequence's
-    // shares does not outweigh summing them
-    const int least = min(most, kWarps * ((int)sqrtf((float)most) / 8 + 1));
+    // shares does not outweigh summing them (1 x 8192 positions, d = 1024: 18.6
+    // us; half as many rounds 21.1, no limit 25.5)
+    const int least = min(most, kWarps * ((int)sqrtf((float)most) / 16 + 1));
     int q = (int)max((units + G - 1) / G, (int64_t)least);
     // even: every item in ceil(nb / q) equal parts of its own, one a CTA, where
-    // that makes no CTA's share longer (64 sequences of 256-511 positions,
-    // d = 512: 22 -> 16.7 us)
+    // that makes no CTA's share much longer (128 sequences of up to 1024
+    // positions, d = 256: 17.6 us, without 19.0; 64 of 256-511, d = 512: 15.2
+    // and 15.5)
     int64_t even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), (int64_t)least) : INT32_MAX;
     const bool even = even_q <= q + 6;
     if (even) q = (int)even_q;
     const int fewer = (q - 1) / (kWarps * RPW) * (kWarps * RPW);
     if (even && p.B <= kThreads && fewer >= max(1, least)) {
         // parts of one round of the warps less, where rounding leaves the CTAs
+        // (64 sequences of 256-511 positions, d = 512: 15.9 -> 15.2 us)
         const int parts = __reduce_add_sync(0xffffffffu, (nb + fewer - 1) / fewer);
         __syncthreads();
         if (lane == 0) s_sum[warp] = parts;
@@ -947,11 +951,14 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                         fm[k] = -INFINITY;
                         fn[k] = fd[k] = 0.f;
                     }
-                    constexpr int kAhead = 8;  // shares whose sums are read at once
-                    for (int g0 = j0; g0 <= j1; g0 += kAhead) {
-                        float x[kAhead][CPT][3];
+                    int g0 = j0;
+                    // the next N shares, whose sums are read at once (8 at a time: 1 x
+                    // 8192 positions, d = 1024, 21.0 us instead of 18.6)
+                    const auto merge = [&](auto count) {
+                        constexpr int N = decltype(count)::value;
+                        float x[N][CPT][3];
 #pragma unroll
-                        for (int d = 0; d < kAhead; ++d) {
+                        for (int d = 0; d < N; ++d) {
                             const float *src = p.part + slot(min(g0 + d, j1)) * 3 * W;
 #pragma unroll
                             for (int k = 0; k < CPT; ++k) {
@@ -962,11 +969,28 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                             }
                         }
 #pragma unroll
-                        for (int d = 0; d < kAhead; ++d)
+                        for (int k = 0; k < CPT; ++k) {
+                            float top = fm[k];
 #pragma unroll
-                            for (int k = 0; k < CPT; ++k)
-                                if (g0 + d <= j1) join(fm[k], fn[k], fd[k], x[d][k][0], x[d][k][1], x[d][k][2]);
-                    }
+                            for (int d = 0; d < N; ++d) top = fmax_nan(top, x[d][k][0]);
+                            if (top == -INFINITY) continue;  // masked so far
+                            const float a = ex2(fm[k] - top);
+                            fn[k] *= a;
+                            fd[k] *= a;
+                            fm[k] = top;
+#pragma unroll
+                            for (int d = 0; d < N; ++d) {
+                                if (g0 + d > j1) continue;
+                                const float c = ex2(x[d][k][0] - top);
+                                fn[k] = fmaf(x[d][k][1], c, fn[k]);
+                                fd[k] = fmaf(x[d][k][2], c, fd[k]);
+                            }
+                        }
+                        g0 += N;
+                    };
+                    while (g0 + 8 <= j1) merge(std::integral_constant<int, 16>{});
+                    if (g0 + 4 <= j1) merge(std::integral_constant<int, 8>{});
+                    else if (g0 <= j1) merge(std::integral_constant<int, 4>{});
                 }
             }
             if (finish) {
@@ -1019,6 +1043,8 @@ static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
 {
     const dim3 grid((unsigned)decode_grid()), block(kThreads);
     constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
+    // a bias for a group where heads allow it (32 sequences of up to 8191
+    // positions, hs = 128: 113 us, a bias for each 8 channels 145)
     auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
     static SmemOnce once[2];
     const cudaError_t e = once[p.hs % 32 == 0].set(kernel, smem);
