@@ -262,7 +262,7 @@ __device__ __forceinline__ f32x2 factors(uint32_t even, uint32_t odd, int j)
                  __uint_as_float(__byte_perm(w, 0x3f000000u, 0x7044u | (k + 1) << 8)));
 }
 
-// Byte offset of the record// Byte offset of the record of slab `slab` at slot (page, row).
+// Byte offset of the record of slab `slab` at slot (page, row).
 __device__ __forceinline__ size_t record(int page, int row, int slab, int nslab, int page_size, int W)
 {
     return (((size_t)page * nslab + slab) * page_size + row) * (size_t)(W * 5 / 4);
@@ -482,9 +482,10 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 // share a bias (NH = 1: the group, else each 8), raised when a bound on y
 // (the group's largest value is low + 15 step) passes it by more than 16.
 //
-// A channel that lies so far below its group that its den is below 2^-90 has
-// lost terms to underflow: its item is then summed again with a running
-// maximum per channel.
+// A channel that lies so far below its group that its den is below 2^-64 may
+// have lost terms to underflow (a scale below 2^-126 becomes 0, and what it
+// scales is at most 2^16 a position): its item is then summed again with a
+// running maximum per channel.
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
 // other, are cut into equal shares of q blocks, one share a CTA, so ragged
@@ -997,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 int lost = 0;
 #pragma unroll
                 for (int k = 0; k < CPT; ++k)
-                    if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-90f) lost = 1;
+                    if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-64f) lost = 1;
                 if (__syncthreads_or(lost)) {
                     resum<W>(p, b, slab, t, part(0));
 #pragma unroll

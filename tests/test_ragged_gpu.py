@@ -383,6 +383,26 @@ def test_aft_decode4_wide_spread(ops):
     h.check()
 
 
+def test_aft_decode4_far_above(ops):
+    """The last key of one channel lies 2^126 above what came before: for the
+    group's other channels, 2^90 below it, that is not yet lost."""
+    T, rng = 1024, np.random.default_rng(9)
+    w = np.zeros((1, T, T), np.float32)
+    w[0, :, 2::4] = w[0, :, 3::4] = 11.05
+    w[0, T - 1, T - 1] = 25.03
+    h = History(ops, rng, 1, 1, 32, T, 16, "f32", [T - 1], w=w)
+    slots = np.full(h.n_pages * 16, -1, np.int32)
+    i = np.arange(T - 1)
+    slots[:T - 1] = h.table[0, i // 16] * 16 + i % 16
+    kv = torch.ones(len(slots), 64, device="cuda")
+    kv[:, :32] = 0
+    ops.kv4_write(kv[:, :32], kv[:, 32:], cu(slots), h.pages)
+    h.qkv[:] = 0
+    h.qkv[0, 32] = 62.34375
+    h.qkv[0, 64:] = -1
+    h.check()
+
+
 def test_aft_decode4_huge_keys(ops):
     """Keys of up to 9e36: each channel takes the value of its largest."""
     rng = np.random.default_rng(13)
