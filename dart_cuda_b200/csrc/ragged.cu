@@ -496,6 +496,9 @@ int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_s
     if (page_size < 8 || page_size > 256 || (page_size & (page_size - 1)))
         return fail(DC_ERR_INVALID, "page_size must be 8, 16, 32, 64, 128 or 256 (got %d)", page_size);
     if ((int64_t)B * ldtab > INT32_MAX) return fail(DC_ERR_INVALID, "B * ldtab must be below 2^31");
+    // the kernel's index into the free list is a sum of two of these
+    if (n_free > INT32_MAX / 2 || ldtab > INT32_MAX / 2)
+        return fail(DC_ERR_INVALID, "n_free and ldtab must be below 2^30");
     if (B == 0) return DC_OK;
     if (!start || !count || !free_pages || !free_head || !free_head_out || !table)
         return fail(DC_ERR_INVALID, "null pointer");

@@ -337,7 +337,8 @@ int dc_kv_cache_fill(const float *qkv, int ldq, int B, int T, int D, float *cach
  * entries of slots [n_slots] that belong to no token become -1.  row_start
  * [B + 1] receives the prefix sums of the counts.  slots and row_start may be
  * NULL.  A token for which there is no page left gets -1 and sets status bit
- * 0x100.  page_size: 8, 16, 32, 64, 128 or 256.  B = 0 does nothing. */
+ * 0x100.  page_size: 8, 16, 32, 64, 128 or 256; n_free and ldtab below
+ * 2^30.  B = 0 does nothing. */
 int dc_page_tables(const int32_t *start, const int32_t *count, int B, int page_size,
                    const int32_t *free_pages, int n_free, const int32_t *free_head,
                    int32_t *free_head_out, int32_t *table, int ldtab, int32_t *slots, int n_slots,

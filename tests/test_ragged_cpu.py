@@ -24,7 +24,8 @@ def tables(L, B=2, page=16, n_free=4, ldtab=3, slots=FAKE, n_slots=8, ld=0, star
 
 @pytest.mark.parametrize("bad", [dict(B=-1), dict(page=7), dict(page=4), dict(page=512), dict(page=24), dict(n_free=-1),
                                  dict(ldtab=0), dict(n_slots=-1), dict(ld=-1), dict(ld=5), dict(start=None),
-                                 dict(table=None), dict(head=None), dict(B=2**20, ldtab=2**12)])
+                                 dict(table=None), dict(head=None), dict(B=2**20, ldtab=2**12),
+                                 dict(n_free=2**30), dict(B=1, ldtab=2**30)])
 def test_page_tables_refuses(L, bad):
     assert tables(L, **bad) == 1 and L.dc_last_error()
     assert tables(L, B=0) == 0
