@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(512) logits_kernel(const __grid_constant__ Log
         for (int i = threadIdx.x; i < p.chunk / 4; i += blockDim.x)
             reinterpret_cast<uint4 *>(hist)[i] = make_uint4(0, 0, 0, 0);
         const int at = p.pos[(int64_t)b * p.pos_stride];
-        const int known = at < 0 ? 0 : min(p.ldt, at + 1);
+        const int known = at < 0 ? 0 : min(p.ldt - 1, at) + 1;
         const int prompt = p.prompt ? p.prompt[b] : 0;
         const int32_t *tok = p.tokens + (int64_t)b * p.ldt;
         __syncthreads();

@@ -572,6 +572,25 @@ def test_logits_controls_not_finite(ops):
     assert y[0] == float("inf") and y[1] == float("-inf") and y[2] != y[2] and y[3] == 0.5 - 2 and y[4] == float("-inf")
 
 
+def test_logits_controls_position_behind_the_row(ops):
+    """Positions past the tokens' capacity, up to the largest int."""
+    tokens = torch.tensor([[1, 2, 2], [1, 2, 2], [1, 2, 2]], dtype=torch.int32, device="cuda")
+    pos = torch.tensor([2, 3, 2**31 - 1], dtype=torch.int32, device="cuda")
+    y = ops.logits_controls(torch.zeros(3, 5, device="cuda"), tokens, pos, frequency=torch.ones(3, device="cuda"))
+    assert y.tolist() == [[0, -1, -2, 0, 0]] * 3
+
+
+def test_single_rows_of_any_stride(ops):
+    """A tensor of one row has no row stride."""
+    rng = np.random.default_rng(21)
+    h = History(ops, rng, 1, 1, 32, 20, 8, "f32", [19])
+    want = h.step().clone()
+    wide = torch.zeros(2, 97, device="cuda")
+    wide[0, :96] = h.qkv[0]
+    h.qkv = wide[:1, :96]
+    assert torch.equal(h.step(), want) and ops.read_status() == 0
+
+
 def test_logits_controls_shared_position(ops):
     rng = np.random.default_rng(2)
     B, V, T = 4, 300, 20
