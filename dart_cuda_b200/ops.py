@@ -336,8 +336,7 @@ def _ld2(t: torch.Tensor) -> int:
     """Row stride of a 2-D tensor (at least the width where there is one row:
     torch gives such a row any stride)."""
     rows, cols = t.shape
-    ld = t.stride()[0]
-    return ld if rows > 1 else max(ld, cols)
+    return t.stride()[0] if rows > 1 else cols
 
 
 def kv4_slab(D: int) -> int:
