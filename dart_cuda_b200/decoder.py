@@ -575,6 +575,8 @@ class AftDecoder:
         if lens is not None and cache_bits != 4:
             raise ValueError("prompts of different lengths need cache_bits=4: the 32-bit history has one position")
         if cache_bits == 4:
+            if page_size < 1:
+                raise ValueError(f"page_size must be positive (got {page_size})")
             lens = [T0] * B if lens is None else [int(n) for n in lens]
             if len(lens) != B or min(lens) < 1 or max(lens) > T0:
                 raise ValueError(f"lens must hold a length of 1..{T0} for each of the {B} prompts")

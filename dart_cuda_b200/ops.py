@@ -333,8 +333,8 @@ def _here(names, *specs):
 
 
 def _ld2(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor (at least the width where there is one row:
-    torch gives such a row any stride)."""
+    """Row stride of a 2-D tensor (the width where there is one row: torch
+    gives such a row any stride)."""
     rows, cols = t.shape
     return t.stride()[0] if rows > 1 else cols
 

@@ -178,7 +178,7 @@ def test_refusals(mods):
     m = model(decoder)
     p = prompts(37, 2, 8)
     for kw in (dict(cache_bits=8), dict(lens=[8, 4]), dict(lens=[8, 9], cache_bits=4), dict(lens=[8, 0], cache_bits=4),
-               dict(lens=[8], cache_bits=4)):
+               dict(lens=[8], cache_bits=4), dict(cache_bits=4, page_size=0)):
         with pytest.raises(ValueError):
             m.prefill(p, **kw)
     with pytest.raises(ValueError):
