@@ -267,9 +267,9 @@ constexpr int kTile = 4;  // logits of a lane in flight
 // warp's lanes side by side so that rows of any alignment are read and
 // written in whole lines.  A larger chunk scans the tokens less often, a
 // smaller one spreads few rows over more SMs.  512 x 50257 bf16 logits, a bias
-// and a mask a row, 2048 known tokens on average, take 50 us (213 MB, 0.66 of
-// the measured copy rate): 41 us without penalties, 6 us for their
-// arithmetic, 3 us for the counting.  Four logits a lane in flight; eight and
+// and a mask a row, 2048 known tokens on average, take 49 us (213 MB, 0.67 of
+// the measured copy rate): 41 us without penalties, the rest their arithmetic
+// and the counting.  Four logits a lane in flight; eight and
 // two were slower (60 us).
 template <typename T>
 __global__ void __launch_bounds__(512) logits_kernel(const __grid_constant__ Logits p)
@@ -281,6 +281,15 @@ __global__ void __launch_bounds__(512) logits_kernel(const __grid_constant__ Log
     const int n = min(p.chunk, p.V - v0);  // chunk: a multiple of 32
     const bool pens = p.rep || p.pres || p.freq;
     if (pens) {
+        // long chunks come into L2 while the tokens are counted (1000 x 32000
+        // fp32: 58 -> 50 us; short ones would wait for the request: 64 x 8192
+        // 3.2 -> 3.4 us).  Whole 16 bytes within the chunk.
+        if (threadIdx.x == 0 && p.chunk > 8192) {
+            const uintptr_t first = reinterpret_cast<uintptr_t>(static_cast<const T *>(p.in) + b * p.ldl + v0);
+            const uintptr_t from = (first + 15) & ~uintptr_t(15), to = (first + n * sizeof(T)) & ~uintptr_t(15);
+            if (from < to)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"((uint32_t)(to - from)) : "memory");
+        }
         for (int i = threadIdx.x; i < p.chunk / 4; i += blockDim.x)
             reinterpret_cast<uint4 *>(hist)[i] = make_uint4(0, 0, 0, 0);
         const int at = p.pos[(int64_t)b * p.pos_stride];

@@ -517,7 +517,7 @@ def test_aft_decode4_captured(ops):
 @pytest.mark.parametrize("B,V,T,dtype,which", [
     (1, 1, 1, "f32", "rpfbm"), (1, 65, 30, "f32", "r"), (3, 97, 200, "bf16", "rpfBM"), (5, 8192, 64, "f32", "rpfbM"),
     (2, 50257, 700, "bf16", "rpfBm"), (4, 4097, 300, "f32", "fb"), (2, 33, 40, "f32", "p"), (3, 20000, 5, "bf16", "M"),
-    (2, 131, 9, "f32", "B"), (2, 64, 9, "f32", "")])
+    (2, 131, 9, "f32", "B"), (2, 64, 9, "f32", ""), (600, 25001, 40, "bf16", "rpfbm"), (600, 17003, 40, "f32", "rf")])
 @pytest.mark.parametrize("ld", [0, 3])
 def test_logits_controls(ops, B, V, T, dtype, which, ld):
     rng = np.random.default_rng(B * V + T)
