@@ -341,6 +341,7 @@ struct Decode {
     int64_t ldtab;
     const int32_t *pos;
     int B, D, hs, W, nslab, n_pages, page_size, cap;
+    float per_hs;  // 1 / hs
     uint32_t page_bytes;
     int shift;  // page_size = 1 << shift
     int w4;  // w's rows start on 16-byte boundaries
@@ -556,22 +557,23 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         most = max(most, s_max[k]);
         active += s_active[k];
     }
-    const int64_t total = (int64_t)sum * p.nslab, items = (int64_t)active * p.nslab;
+    // the plan fits 32 bits (the entry point sees to it): divisions of 64 took
+    // 1 us of a call
+    const int total = sum * p.nslab, items = active * p.nslab;
     if (items == 0) return;
-    const int64_t units = total + items * kItem;
-    const int G = gridDim.x;
+    const int units = total + items * kItem, G = gridDim.x;
     // at least some rounds of the CTA's warps, so that merging a long sequence's
     // shares does not outweigh summing them (1 x 8192 positions, d = 1024: 18.6
     // us; half as many rounds 21.1, no limit 25.5)
     const int least = min(most, kWarps * ((int)sqrtf((float)most) / 16 + 1));
-    int q = (int)max((units + G - 1) / G, (int64_t)least);
+    int q = max((units + G - 1) / G, least);
     // even: every item in ceil(nb / q) equal parts of its own, one a CTA, where
     // that makes no CTA's share much longer (128 sequences of up to 1024
     // positions, d = 256: 17.6 us, without 19.0; 64 of 256-511, d = 512: 15.2
     // and 15.5)
-    int64_t even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), (int64_t)least) : INT32_MAX;
+    const int even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), least) : INT32_MAX;
     const bool even = even_q <= q + 6;
-    if (even) q = (int)even_q;
+    if (even) q = even_q;
     const int fewer = (q - 1) / (kWarps * RPW) * (kWarps * RPW);
     if (even && p.B <= kThreads && fewer >= max(1, least)) {
         // parts of one round of the warps less, where rounding leaves the CTAs
@@ -583,16 +585,16 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
         int all = 0;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) all += s_sum[k];
-        if ((int64_t)all * p.nslab <= G) q = fewer;
+        if (all * p.nslab <= G) q = fewer;
     }
     auto weight = [&](int nb) {  // CTAs, or blocks and what an item costs besides
         return nb == 0 ? 0 : even ? (nb + q - 1) / q : nb + kItem;
     };
     // this CTA's share: [u, u1) of all slabs' weights, one sequence after the other
-    int64_t u = even ? blockIdx.x : (int64_t)blockIdx.x * q;
-    int64_t u1 = even ? u + 1 : min(units, u + q);
+    int u = even ? blockIdx.x : blockIdx.x * q;
+    int u1 = even ? u + 1 : min(units, u + q);
     // the sequence that u lies in: the weight before it
-    const int64_t target = u / p.nslab;
+    const int target = u / p.nslab;
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += kThreads) {
         if (p.B > kThreads) {
@@ -627,26 +629,28 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     if (b < 0) return;  // behind the last share
     t = s_t;
     nb = row_blocks(p, t);
-    const int local = (int)(u - (int64_t)s_first * p.nslab), own = weight(nb);
+    const int local = u - s_first * p.nslab, own = weight(nb);
     int slab = local / own, off = local % own;  // off: units of the item before the share
     int j0 = blockIdx.x - off, j1 = j0 + own - 1;
     if (even) {  // part off of own: its blocks, as units behind the item's kItem
-        u1 = kItem + (int64_t)(off + 1) * nb / own;
-        off = kItem + (int)((int64_t)off * nb / own);
+        u1 = kItem + (uint32_t)((off + 1) * nb) / (uint32_t)own;
+        off = kItem + (uint32_t)(off * nb) / (uint32_t)own;
         u = off;
     }
 
     for (;;) {
-        const int taken = (int)min((int64_t)(nb + kItem - off), u1 - u);
+        const int taken = min(nb + kItem - off, u1 - u);
         const int blk = max(0, off - kItem), n = off + taken - kItem - blk;  // the share's blocks
-        const int64_t u_item = u - off;
+        const int u_item = u - off;
         if (n > 0) {
             const int32_t *tab = p.table + b * p.ldtab;
             const T *row = static_cast<const T *>(p.qkv) + b * p.ldq + slab * W;
+            // exact below 2^21
+            auto head_of = [&](int channel) { return (int)((channel + 0.5f) * p.per_hs); };
             const float *w[NH];  // bias rows of this lane's octets
 #pragma unroll
             for (int h = 0; h < NH; ++h)
-                w[h] = p.w + ((slab * W + group * 32 + (h ^ (2 * flip)) * 8 * (NH > 1)) / p.hs) * p.wh + t * p.ldw + rq;
+                w[h] = p.w + head_of(slab * W + group * 32 + (h ^ (2 * flip)) * 8 * (NH > 1)) * p.wh + t * p.ldw + rq;
             // this warp's blocks: k0, k0 + step, ... < n, RPW neighbours at once
             constexpr int kStep = kWarps * RPW;
             const int k0 = warp * RPW + sub;
@@ -925,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             bool finish = n == nb;
             if (!finish) {  // shared with other CTAs
                 // second slot: an item that begins inside the CTA's share
-                const auto slot = [&](int g) { return (int64_t)g * 2 + (!even && u_item > (int64_t)g * q); };
+                const auto slot = [&](int g) { return (int64_t)g * 2 + (!even && u_item > g * q); };
                 float *mine = p.part + slot(blockIdx.x) * 3 * W;
 #pragma unroll
                 for (int k = 0; k < CPT; ++k) {
@@ -938,8 +942,8 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 __threadfence();
                 __syncthreads();
                 if (!even) {
-                    j0 = (int)((u_item + kItem) / q);
-                    j1 = (int)((u_item + kItem + nb - 1) / q);
+                    j0 = (u_item + kItem) / q;
+                    j1 = (u_item + kItem + nb - 1) / q;
                 }
                 if (tid == 0) {
                     int *counter = p.counter + (int64_t)b * p.nslab + slab;
@@ -1184,6 +1188,7 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     p.B = B;
     p.D = D;
     p.hs = hs;
+    p.per_hs = 1.f / hs;
     p.W = slab_width(D);
     p.nslab = D / p.W;
     p.n_pages = n_pages;
@@ -1196,10 +1201,12 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
     p.counter = reinterpret_cast<int *>(static_cast<char *>(workspace) + part_bytes());
     p.Z = Z;
     p.ldz = ldz;
+    // the kernel's plan in 32 bits
+    const int blocks = p.cap / kRows + 1;
+    if (blocks > 65536 || (double)B * p.nslab * (blocks + kItem) > (1 << 30))
+        return fail(DC_ERR_INVALID, "Tmax must be below 2^20, and B * D * Tmax is limited (B=%d D=%d Tmax=%d)", B, D, Tmax);
     p.status = device_status_word();
     if (!p.status) return fail(DC_ERR_CUDA, "no device status word");
-    if ((int64_t)B * (p.cap / kRows + 1 + kItem) > INT32_MAX || (int64_t)B * p.nslab > INT32_MAX / 4)
-        return fail(DC_ERR_INVALID, "B * Tmax or B * D too large");
     cudaStream_t st = as_stream(stream);
     KernelTimer kt("aft_decode4", st);
     DC_CUDA_TRY(dtype == DC_F32 ? launch_decode<float>(p, st) : launch_decode<__nv_bfloat16>(p, st));

@@ -372,9 +372,9 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
  * receives the AFT row over the positions 0..t that the history then holds.
  * w is head h's bias at w + h * head_stride_w, row stride ldw >= Tmax.  A
  * sequence with pos < 0 is left out and its Z row is zero; so is one with
- * pos >= min(Tmax, ldtab * page_size), which sets status bit 0x40, and one
- * whose bias row is -inf throughout.  Sequences may share pages they only
- * read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
+ * pos >= c = min(Tmax, ldtab * page_size), which sets status bit 0x40, and one
+ * whose bias row is -inf throughout.  c is below 2^20, and B * D/W * (c/16 +
+ * 11) at most 2^30.  Sequences may share pages they only read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
  * zero-filled once before its first use (the kernel leaves its counters
  * zeroed), for this or any smaller B and D; calls that may overlap on the GPU
  * need one each. */

@@ -51,6 +51,7 @@ def decode(L, qkv=FAKE, ldq=192, dtype=0, w=FAKE, ldw=32, pages=FAKE, n_pages=9,
 
 
 @pytest.mark.parametrize("bad", [dict(B=-1), dict(H=0), dict(hs=0), dict(hs=12), dict(hs=4, H=16), dict(H=1, hs=24),
+                                 dict(Tmax=2**20, ldw=2**20, ldtab=2**18), dict(B=2**20, Tmax=2**15, ldw=2**15, ldtab=2**12),
                                  dict(H=2**20, hs=2**12), dict(Tmax=0), dict(ldtab=0), dict(dtype=7), dict(ldq=188),
                                  dict(ldq=194), dict(ldz=63), dict(ldz=68, dtype=1), dict(ldw=31), dict(page=9),
                                  dict(n_pages=0), dict(qkv=None), dict(w=None), dict(pages=None), dict(table=None),
