@@ -286,9 +286,9 @@ constexpr int kWriteWarps = 4;
 // 256 channels of a row (blockIdx.y which of them), or 32/span rows of fewer.
 // Rows with a negative slot are left out.  Bound by HBM and issue alike: 65521
 // rows of 2048 bf16 channels with their values back, 1.24 GB, take 264 us
-// (0.73 of the measured copy rate), about 25 instructions a value, a fifth of
-// them for borders, which bf16 values meet often; with a division for the
-// step and one a value it took 702 us.
+// (0.73 of the measured copy rate), about 25 instructions a value, part of them
+// for borders, which bf16 values meet often; with a division for the step and
+// one a value it took 702 us.
 template <typename T>
 __global__ void __launch_bounds__(32 * kWriteWarps, 9) write_kernel(const __grid_constant__ Write p, int span)
 {
@@ -498,9 +498,9 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 // What bounds it: a channel of a position costs one 2^x (8 cycles a warp and
 // scheduler) and about 7 other instructions that overlap with it imperfectly
 // (9.5 cycles alone), against 1.25 bytes of HBM, so 32 sequences of up to 8191
-// positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 113 us; the
+// positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 111 us; the
 // rest is what an item costs besides (merging, its first loads).  At 64
-// sequences of 256-511 positions, d = 512, these are most of the 15 us.  Steps
+// sequences of 256-511 positions, d = 512, these are most of the 14.5 us.  Steps
 // there: a lane per 8 channels 146 us (10.5 instructions a channel for
 // unpacking and bounds), 16 channels 183 us (too few registers), a group of 32
 // by four rows 141 us; codes through mixed-precision bf16 FMAs instead of byte
@@ -563,14 +563,13 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     if (items == 0) return;
     const int units = total + items * kItem, G = gridDim.x;
     // at least some rounds of the CTA's warps, so that merging a long sequence's
-    // shares does not outweigh summing them (1 x 8192 positions, d = 1024: 18.6
-    // us; half as many rounds 21.1, no limit 25.5)
+    // shares does not outweigh summing them (1 x 8192 positions, d = 1024: 18.2
+    // us; half as many rounds 21.1)
     const int least = min(most, kWarps * ((int)sqrtf((float)most) / 16 + 1));
     int q = max((units + G - 1) / G, least);
     // even: every item in ceil(nb / q) equal parts of its own, one a CTA, where
     // that makes no CTA's share much longer (128 sequences of up to 1024
-    // positions, d = 256: 17.6 us, without 19.0; 64 of 256-511, d = 512: 15.2
-    // and 15.5)
+    // positions, d = 256: 17.6 us, without 19.0)
     const int even_q = 2 * items <= G ? max((total + G - items - 1) / (G - items), least) : INT32_MAX;
     const bool even = even_q <= q + 6;
     if (even) q = even_q;
@@ -1051,7 +1050,7 @@ static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
     const dim3 grid((unsigned)decode_grid()), block(kThreads);
     constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
     // a bias for a group where heads allow it (32 sequences of up to 8191
-    // positions, hs = 128: 113 us, a bias for each 8 channels 145)
+    // positions, hs = 128: 114 us, a bias for each 8 channels 145)
     auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
     static SmemOnce once[2];
     const cudaError_t e = once[p.hs % 32 == 0].set(kernel, smem);
