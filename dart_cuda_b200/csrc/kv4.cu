@@ -402,23 +402,34 @@ __device__ __forceinline__ void join(float &m, float &num, float &den, float m2,
     m = mx;
 }
 
-// The sums of one item with a running maximum per channel, by the whole CTA,
-// from the stored history (position t appended): num [W], den [W] into out.
-// out holds 3 * W * kWarps floats.
+// One item again with a running maximum per channel and sums in 64 bits, which
+// no value and no number of positions overflows, by the whole CTA from the
+// stored history (position t appended).  out holds (5 * kWarps + 1) * W floats;
+// returns the W weighted means that it leaves there (0 where the bias masks
+// every position).
 template <int W>
-__device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, float *out)
+__device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int t, float *out)
 {
     constexpr int LPR = W / 8, RPW = 32 / LPR;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LPR, oct = lane % LPR;
     const int ch = slab * W + oct * 8;
     const int32_t *tab = p.table + b * p.ldtab;
     const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
-    float m[8], num[8], den[8];
+    float m[8];
+    double num[8], den[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         m[j] = -INFINITY;
-        num[j] = den[j] = 0.f;
+        num[j] = den[j] = 0.;
     }
+    auto add = [](float &m, double &num, double &den, float m2, double num2, double den2) {
+        const float mx = fmax_nan(m, m2);
+        if (mx == -INFINITY) return;  // masked so far
+        const float a = ex2((m - mx) * kLog2e), c = ex2((m2 - mx) * kLog2e);
+        num = num * a + num2 * c;
+        den = den * a + den2 * c;
+        m = mx;
+    };
     for (int i = warp * RPW + sub; i <= t; i += kWarps * RPW) {
         const int page = tab[i >> p.shift];
         if (page < 0 || page >= p.n_pages) continue;
@@ -430,48 +441,37 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
         values8(code.x, par.x, k);
         values8(code.y, par.y, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = k[j] + wi;
-            const float mx = fmax_nan(m[j], x);
-            if (mx == -INFINITY) continue;  // masked so far
-            const float scale = ex2((m[j] - mx) * kLog2e), e = ex2((x - mx) * kLog2e);
-            num[j] = num[j] * scale + e * v[j];
-            den[j] = den[j] * scale + e;
-            m[j] = mx;
-        }
+        for (int j = 0; j < 8; ++j) add(m[j], num[j], den[j], k[j] + wi, v[j], 1.);
     }
-    auto add = [](float &m, float &num, float &den, float m2, float num2, float den2) {
-        const float mx = fmax_nan(m, m2);
-        if (mx == -INFINITY) return;
-        const float a = ex2((m - mx) * kLog2e), c = ex2((m2 - mx) * kLog2e);
-        num = num * a + num2 * c;
-        den = den * a + den2 * c;
-        m = mx;
-    };
 #pragma unroll
     for (int o = LPR; o < 32; o *= 2)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o), n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
+            const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o);
+            const double n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
             add(m[j], num[j], den[j], m2, n2, __shfl_xor_sync(0xffffffffu, den[j], o));
         }
+    // [kWarps][W] numerators, denominators, maxima; then the means [W]
+    double *nums = reinterpret_cast<double *>(out), *dens = nums + kWarps * W;
+    float *tops = reinterpret_cast<float *>(dens + kWarps * W), *mean = tops + kWarps * W;
     __syncthreads();
     if (sub == 0) {
-        store8(out + (warp * 3 + 0) * W + oct * 8, num);
-        store8(out + (warp * 3 + 1) * W + oct * 8, den);
-        store8(out + (warp * 3 + 2) * W + oct * 8, m);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            nums[warp * W + oct * 8 + j] = num[j];
+            dens[warp * W + oct * 8 + j] = den[j];
+            tops[warp * W + oct * 8 + j] = m[j];
+        }
     }
     __syncthreads();
     for (int c = threadIdx.x; c < W; c += kThreads) {
-        float mc = out[2 * W + c], nc = out[c], dc = out[W + c];
-        for (int g = 1; g < kWarps; ++g) {
-            const float *src = out + g * 3 * W + c;
-            add(mc, nc, dc, src[2 * W], src[0], src[W]);
-        }
-        out[c] = nc;
-        out[W + c] = dc;
+        float mc = tops[c];
+        double nc = nums[c], dc = dens[c];
+        for (int g = 1; g < kWarps; ++g) add(mc, nc, dc, tops[g * W + c], nums[g * W + c], dens[g * W + c]);
+        mean[c] = dc == 0. ? 0.f : (float)(nc / dc);
     }
     __syncthreads();
+    return mean;
 }
 
 // The history of a slab (W channels of one sequence) is read once, in blocks
@@ -485,8 +485,10 @@ __device__ __noinline__ void resum(const Decode &p, int b, int slab, int t, floa
 //
 // A channel that lies so far below its group that its den is below 2^-64 may
 // have lost terms to underflow (a scale below 2^-126 becomes 0, and what it
-// scales is at most 2^16 a position): its item is then summed again with a
-// running maximum per channel.
+// scales is at most 2^16 a position), and values may be so large (up to 1e37
+// times a weight of up to 2^16) that num overflows, which leaves it infinite or
+// NaN beside a finite den: such an item is then summed again, in 64 bits and
+// with a running maximum per channel.
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
 // other, are cut into equal shares of q blocks, one share a CTA, so ragged
@@ -524,6 +526,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     auto ring = reinterpret_cast<uint8_t(*)[kStages][kStageBytes]>(ring_raw);
     auto part = [&](int warp) { return reinterpret_cast<float *>(ring[warp][0]); };
     static_assert(kStages * kStageBytes >= 8 * 1024, "room for the lanes' sums");
+    static_assert(kWarps * kStages * kStageBytes >= (5 * kWarps + 1) * W * 4, "room for resum's");
     const uint32_t mine = smem_u32(ring[warp][0]) + sub * (kRows * kRec) + oct * 16;
     __shared__ int s_sum[kWarps], s_max[kWarps], s_active[kWarps], s_b, s_first, s_t, s_last;
 
@@ -1003,16 +1006,18 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             if (finish) {
                 int lost = 0;
 #pragma unroll
-                for (int k = 0; k < CPT; ++k)
-                    if (tid + k * kThreads < W && fm[k] != -INFINITY && fd[k] < 0x1p-64f) lost = 1;
+                for (int k = 0; k < CPT; ++k) {
+                    if (tid + k * kThreads >= W || fm[k] == -INFINITY) continue;
+                    if (fd[k] < 0x1p-64f || (fd[k] < INFINITY && !(fabsf(fn[k]) < INFINITY))) lost = 1;
+                }
                 if (__syncthreads_or(lost)) {
-                    resum<W>(p, b, slab, t, part(0));
+                    const float *mean = resum<W>(p, b, slab, t, part(0));
 #pragma unroll
                     for (int k = 0; k < CPT; ++k) {
                         const int c = tid + k * kThreads;
                         if (c >= W) continue;
-                        fn[k] = part(0)[c];
-                        fd[k] = part(0)[W + c];
+                        fn[k] = mean[c];
+                        fd[k] = 1.f;
                     }
                 }
 #pragma unroll
