@@ -243,11 +243,11 @@ __device__ __forceinline__ uint32_t pack_params(float step, float low)
 }
 
 // The 8 values that codes stand for.
-__device__ __forceinline__ void values8(uint32_t codes, uint32_t params, float (&x)[8])
+__device__ __forceinline__ void values8(uint32_t codes, uint32_t params, double (&x)[8])
 {
-    const float step = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
+    const double step = __uint_as_float(params << 16), low = __uint_as_float(params & 0xffff0000u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fmaf(step, (float)((codes >> (4 * j)) & 15u), low);
+    for (int j = 0; j < 8; ++j) x[j] = fma(step, (double)((codes >> (4 * j)) & 15u), low);
 }
 
 // Two codes as fp32 numbers 1/2 + c/32: the codes of a word are masked into
@@ -372,6 +372,12 @@ __device__ __forceinline__ float fmax_nan(float a, float b)
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kResident = 3;
 constexpr int kRows = 16;  // history rows of a block: two halves, each within a page
 constexpr int kStages = 2;  // blocks in flight of a warp
+constexpr float kHuge = 0x1p24f;  // exponents of this size have no fraction in fp32
+// (low - 16 step)^2 + step^2 of a row with a key of 2^23 or more is above this;
+// a lane's sum of them may reach it from somewhat smaller keys on.  Summed
+// packed (a maximum a row instead: 113.0 instead of 110.3 us at 32 x <=8191).
+constexpr float kFar = 0x1p36f;
+constexpr float kAbsorbs = 1e30f;  // beside a finite bias of this size keys below 2^23 vanish, in 64 bits too
 constexpr int kItem = 10;   // what an item costs a CTA besides its blocks, in blocks
 
 // 16 bytes, of which the first `bytes` (0 or 16) are read, the others zeros
@@ -402,11 +408,11 @@ __device__ __forceinline__ void join(float &m, float &num, float &den, float m2,
     m = mx;
 }
 
-// One item again with a running maximum per channel and sums in 64 bits, which
-// no value and no number of positions overflows, by the whole CTA from the
-// stored history (position t appended).  out holds (5 * kWarps + 1) * W floats;
-// returns the W weighted means that it leaves there (0 where the bias masks
-// every position).
+// One item again with a running maximum per channel, exponents and sums in 64
+// bits, which no value, bias or number of positions overflows, by the whole
+// CTA from the stored history (position t appended).  out holds (6 * kWarps +
+// 1) * W floats; returns the W weighted means that it leaves there (0 where
+// the bias masks every position).
 template <int W>
 __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int t, float *out)
 {
@@ -415,17 +421,16 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
     const int ch = slab * W + oct * 8;
     const int32_t *tab = p.table + b * p.ldtab;
     const float *w = p.w + (ch / p.hs) * p.wh + t * p.ldw;
-    float m[8];
-    double num[8], den[8];
+    double m[8], num[8], den[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         m[j] = -INFINITY;
         num[j] = den[j] = 0.;
     }
-    auto add = [](float &m, double &num, double &den, float m2, double num2, double den2) {
-        const float mx = fmax_nan(m, m2);
-        if (mx == -INFINITY) return;  // masked so far
-        const float a = ex2((m - mx) * kLog2e), c = ex2((m2 - mx) * kLog2e);
+    auto add = [](double &m, double &num, double &den, double m2, double num2, double den2) {
+        const double mx = m2 > m || m2 != m2 ? m2 : m;  // NaN if either is
+        if (mx == -INFINITY) return;                    // masked so far
+        const float a = ex2((float)((m - mx) * 1.4426950408889634)), c = ex2((float)((m2 - mx) * 1.4426950408889634));
         num = num * a + num2 * c;
         den = den * a + den2 * c;
         m = mx;
@@ -436,8 +441,8 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
         const uint8_t *rec = p.pages + record(page, i & (p.page_size - 1), slab, p.nslab, p.page_size, W);
         const uint2 code = *reinterpret_cast<const uint2 *>(rec + oct * 8);
         const uint2 par = *reinterpret_cast<const uint2 *>(rec + W + oct / 4 * 8);
-        const float wi = w[i];
-        float k[8], v[8];
+        const double wi = w[i];
+        double k[8], v[8];
         values8(code.x, par.x, k);
         values8(code.y, par.y, v);
 #pragma unroll
@@ -447,13 +452,12 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
     for (int o = LPR; o < 32; o *= 2)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o);
-            const double n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
+            const double m2 = __shfl_xor_sync(0xffffffffu, m[j], o), n2 = __shfl_xor_sync(0xffffffffu, num[j], o);
             add(m[j], num[j], den[j], m2, n2, __shfl_xor_sync(0xffffffffu, den[j], o));
         }
     // [kWarps][W] numerators, denominators, maxima; then the means [W]
-    double *nums = reinterpret_cast<double *>(out), *dens = nums + kWarps * W;
-    float *tops = reinterpret_cast<float *>(dens + kWarps * W), *mean = tops + kWarps * W;
+    double *nums = reinterpret_cast<double *>(out), *dens = nums + kWarps * W, *tops = dens + kWarps * W;
+    float *mean = reinterpret_cast<float *>(tops + kWarps * W);
     __syncthreads();
     if (sub == 0) {
 #pragma unroll
@@ -465,8 +469,7 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
     }
     __syncthreads();
     for (int c = threadIdx.x; c < W; c += kThreads) {
-        float mc = tops[c];
-        double nc = nums[c], dc = dens[c];
+        double mc = tops[c], nc = nums[c], dc = dens[c];
         for (int g = 1; g < kWarps; ++g) add(mc, nc, dc, tops[g * W + c], nums[g * W + c], dens[g * W + c]);
         mean[c] = dc == 0. ? 0.f : (float)(nc / dc);
     }
@@ -488,7 +491,11 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
 // scales is at most 2^16 a position), and values may be so large (up to 1e37
 // times a weight of up to 2^16) that num overflows, which leaves it infinite or
 // NaN beside a finite den: such an item is then summed again, in 64 bits and
-// with a running maximum per channel.
+// with a running maximum per channel.  So are those whose exponents fp32 does
+// not hold: references from 2^24 on (a row masked throughout by -1e9) and keys
+// from 2^23 on, which a bias of their size may cancel.  Beside smaller keys a
+// finite bias from 1e30 on (a mask of the type's lowest value) is the whole of
+// the sum in 64 bits too, and the keys are left out.
 //
 // Work split: the row blocks of all (sequence, slab) items, one after the
 // other, are cut into equal shares of q blocks, one share a CTA, so ragged
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
     auto ring = reinterpret_cast<uint8_t(*)[kStages][kStageBytes]>(ring_raw);
     auto part = [&](int warp) { return reinterpret_cast<float *>(ring[warp][0]); };
     static_assert(kStages * kStageBytes >= 8 * 1024, "room for the lanes' sums");
-    static_assert(kWarps * kStages * kStageBytes >= (5 * kWarps + 1) * W * 4, "room for resum's");
+    static_assert(kWarps * kStages * kStageBytes >= (6 * kWarps + 1) * W * 4, "room for resum's");
     const uint32_t mine = smem_u32(ring[warp][0]) + sub * (kRows * kRec) + oct * 16;
     __shared__ int s_sum[kWarps], s_max[kWarps], s_active[kWarps], s_b, s_first, s_t, s_last;
 
@@ -728,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             // octet o, pair j (factors)
             f32x2 num[4][4], den[4][4];
             float ref[NH];
+            f32x2 far = 0;  // sums of the keys' (low - 16 step)^2 and step^2
 #pragma unroll
             for (int o = 0; o < 4; ++o)
 #pragma unroll
@@ -763,6 +771,12 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                     }
                     __syncwarp();
                 }
+                // one test for the four rows (112.1 -> 109.5 us at 32 x <=8191
+                // positions; with four biases a row one each is as fast)
+                bool odd = false;
+#pragma unroll
+                for (int h = 0; h < NH; ++h)
+                    odd |= fmaxf(fmaxf(fabsf(wl[h].x), fabsf(wl[h].y)), fmaxf(fabsf(wl[h].z), fabsf(wl[h].w))) >= kAbsorbs;
                 // rows whose exponents are bounded together: fewer branches between
                 // the sums (two with one bias a row: 116.6 -> 113 us; else one, for registers)
                 constexpr int kTogether = NH == 1 ? 2 : 1;
@@ -782,16 +796,16 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                         const float klow = fmaf(kstep, -16.f, __uint_as_float(par.x & 0xffff0000u));
                         va[i] = fmaf(vstep, -16.f, __uint_as_float(par.y & 0xffff0000u));
                         vs[i] = 32.f * vstep;
+                        far = fma2(pack2(klow, kstep), pack2(klow, kstep), far);
 #pragma unroll
                         for (int h = 0; h < NH; ++h) {
                             const float x = r == 0 ? wl[h].x : r == 1 ? wl[h].y : r == 2 ? wl[h].z : wl[h].w;
                             ks[i][h] = kstep * (32.f * kLog2e);
-                            ka[i][h] = fmaf(klow, kLog2e, x * kLog2e);
-                            if (fabsf(x) >= 1e30f && fabsf(x) < INFINITY) {
-                                // a finite bias of such size (a mask of -FLT_MAX)
-                                // absorbs the keys, in fp32 as in 64 bits
+                            ka[i][h] = (klow + x) * kLog2e;
+                            if ((NH > 1 || odd) && fabsf(x) >= kAbsorbs && x > -INFINITY) {
+                                // any factor serves that keeps it finite
                                 ks[i][h] = 0.f;
-                                ka[i][h] = fminf(fmaxf(x * kLog2e, -3.4028234e38f), 3.4028234e38f);
+                                ka[i][h] = 0.5f * x;
                             }
                             top[h] = fmax_nan(top[h], fmaf(ks[i][h], 31.f / 32.f, ka[i][h]));
                         }
@@ -866,6 +880,8 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
             float *sums = part(warp);  // [NL][2][W], then ref, num, den [3][W]
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
+                const float keys = unpack2(far).x + unpack2(far).y;
+                if (!(keys < kFar)) ref[h] = keys * INFINITY;  // or NaN, which reaches Z
                 float r = ref[h];
 #pragma unroll
                 for (int x = NG; x < 32; x *= 2) r = fmax_nan(r, __shfl_xor_sync(0xffffffffu, r, x));
@@ -1004,11 +1020,13 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                 }
             }
             if (finish) {
-                int lost = 0;
+                bool lost = false;
 #pragma unroll
                 for (int k = 0; k < CPT; ++k) {
                     if (tid + k * kThreads >= W || fm[k] == -INFINITY) continue;
-                    if (fd[k] < 0x1p-64f || (fd[k] < INFINITY && !(fabsf(fn[k]) < INFINITY))) lost = 1;
+                    const float far = fabsf(fm[k]);
+                    lost |= (far >= kHuge && far < 0.5f * kAbsorbs) || far == INFINITY || fd[k] < 0x1p-64f ||
+                            (fd[k] < INFINITY && !(fabsf(fn[k]) < INFINITY));
                 }
                 if (__syncthreads_or(lost)) {
                     const float *mean = resum<W>(p, b, slab, t, part(0));

@@ -85,3 +85,44 @@ def test_aft_decode4_huge_values(ops, H, hs, kind):
         h.qkv[:, D: 2 * D] = 0
     got = check(h, 20)
     assert np.isfinite(got).all() and np.abs(got[0, :32]).max() > 1e33
+
+
+LOWEST = float(np.finfo(np.float32).min)
+
+
+@pytest.mark.parametrize("H,hs", SHAPES)
+@pytest.mark.parametrize("kind", ["absorbed", "levels", "above", "cancel", "nan", "row", "below", "shares"])
+def test_aft_decode4_huge_bias(ops, H, hs, kind):
+    """Finite biases beside which fp32 holds nothing of a key, and keys that
+    outweigh them all the same: exponents are the sums in 64 bits."""
+    rng = np.random.default_rng(H * hs + 1)
+    D, T = H * hs, 900 if kind == "shares" else 120
+    lens = [T - 1] if kind == "shares" else [T - 1, 70]
+    w = (0.5 * rng.standard_normal((H, T, T))).astype(np.float32)
+    kv = rng.standard_normal((len(lens), T, 2 * D))
+    key = kv[..., :32]  # one group, beside ordinary ones
+    if kind == "absorbed":
+        w[:] = 1e30
+        kv[..., :32] = 2e36 * key
+    elif kind in ("levels", "shares"):  # every position masked, some of them less
+        w[:] = LOWEST
+        w[:, :, 5::7] = -3e38
+    elif kind == "above":
+        w[:, :, ::3] = -1e30
+        kv[..., :32] = 1e33 * key
+    elif kind == "cancel":
+        w[:, :, 5] = -2.0**119
+        kv[:, 5, :32] = 2.0**119
+    elif kind == "nan":
+        w[:, :, 5] = LOWEST
+        kv[0, 5, 3] = np.nan
+    elif kind == "row":
+        w[:] = -1e9
+    elif kind == "below":
+        w[:] = LOWEST
+        kv[..., :32] = -9e36 * np.abs(key) / np.abs(key).max()
+    h = History(ops, rng, len(lens), H, hs, T, 8, "f32", lens, w=w)
+    store(h, kv)
+    got = check(h, 20)
+    if kind == "nan":
+        assert np.isnan(got).sum() == 32
