@@ -86,26 +86,53 @@ class LogitControls:
     one per sequence; bias: [V] or [B, V] fp32; mask: packed int32 words
     [ceil(V/32)] or [B, ceil(V/32)], bit set = token allowed.  The presence and
     frequency penalties count generated tokens, the repetition penalty the
-    prompt's too.  A mask or bias on the device may be rewritten between
-    steps."""
+    prompt's too.  Tensors on the device (fp32, int32 for the mask) are read at
+    every step and may be rewritten between steps; what else is given is copied
+    by ``prefill``."""
     repetition: object = None
     presence: object = None
     frequency: object = None
     bias: torch.Tensor | None = None
     mask: torch.Tensor | None = None
 
-    def on(self, B, device):
-        """Keyword arguments of ops.logits_controls for B sequences."""
-        def rows(x):
+    def on(self, B, device, kept):
+        """Keyword arguments of ops.logits_controls for B sequences.  Copies
+        lie in the tensors of ``kept`` (by name), the same for every call that
+        fits them, so that a captured step reads the last call's."""
+        def put(name, x, dtype=None, rows=None):
             if x is None:
                 return None
-            return torch.as_tensor(x, dtype=torch.float32, device=device).expand(B).contiguous()
+            x = torch.as_tensor(x, dtype=dtype)
+            y = x.to(device)
+            if rows is not None:
+                y = y.expand(rows).contiguous()
+            if y.data_ptr() == x.data_ptr():
+                return y  # the caller's own
+            if name not in kept or kept[name].shape != y.shape or kept[name].dtype != y.dtype:
+                kept[name] = torch.empty_like(y)
+            return kept[name].copy_(y)
 
-        def put(x):
-            return None if x is None else x.to(device)
+        out = {name: put(name, getattr(self, name), torch.float32, B) for name in ("repetition", "presence", "frequency")}
+        return dict(out, bias=put("bias", self.bias), mask=put("mask", self.mask))
 
-        return dict(repetition=rows(self.repetition), presence=rows(self.presence), frequency=rows(self.frequency),
-                    bias=put(self.bias), mask=put(self.mask))
+
+class DecodeGraph(torch.cuda.CUDAGraph):
+    """A captured decode step (``AftDecoder.capture_decode_step``).  It replays
+    on the buffers that it was captured with, across prefills that use the same
+    ones; ``replay`` raises when the model's last prefill took others (another
+    batch size or history, a larger pool, other kinds of controls)."""
+
+    def bind(self, model):
+        self.model, self.state = model, model._dec
+        self.decode_state = dict(model._dec)  # what it replays on lives as long as it
+        self.controls = model._controls_key()
+        return self
+
+    def replay(self):
+        if self.model._dec is not self.state or self.model._controls_key() != self.controls:
+            raise RuntimeError("the last prefill uses another history or other controls than this graph was captured "
+                               "with: capture the decode step again")
+        super().replay()
 
 
 class AftDecoder:
@@ -529,7 +556,7 @@ class AftDecoder:
         d, F, Tm = c.d_model, c.ffn_mult * c.d_model, c.block_size
         z = lambda *s: torch.zeros(*s, device=dev)
         zi = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
-        s = {"B": B, "key": key, "controls": None}
+        s = {"B": B, "key": key, "controls": None, "kept": {}}
         s["x"], s["a"], s["zd"], s["cg"] = (z(B, d) for _ in range(4))
         s["qkv"], s["h"] = z(B, 3 * d), z(B, F)
         s["logits"] = z(B, c.vocab)
@@ -586,7 +613,7 @@ class AftDecoder:
         else:
             s = self._decode_state(B)
             s["prompt_len"].fill_(T0)
-        s["controls"] = None if controls is None else controls.on(B, self.device)
+        s["controls"] = None if controls is None else controls.on(B, self.device, s["kept"])
         st = ops._stream()
         if cache_bits == 4:
             s["head"].zero_()
@@ -700,11 +727,17 @@ class AftDecoder:
                     self.decode_step()
         return self._dec["tokens"][:, : T0 + n_new]
 
+    def _controls_key(self):
+        """Which tensors a decode step takes its controls from."""
+        c = self._dec["controls"]
+        return c and {k: t if t is None else (t.data_ptr(), t.shape, t.stride()) for k, t in c.items()}
+
     def capture_decode_step(self):
         """A CUDA graph of one decode step.  Capturing does not run it; each
-        replay decodes the position held in device memory and advances it."""
-        g = torch.cuda.CUDAGraph()
+        replay decodes the position held in device memory and advances it.  It
+        may be kept across prefills; one that needs another graph makes its
+        replay raise (``DecodeGraph``)."""
+        g = DecodeGraph()
         with torch.cuda.graph(g):
             self.decode_step()
-        g.decode_state = dict(self._dec)  # the buffers it replays on live as long as it
-        return g
+        return g.bind(self)
