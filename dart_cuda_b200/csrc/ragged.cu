@@ -564,6 +564,8 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
 {
     clear_error();
     if (B < 0 || V <= 0 || ldl < V || ldo < V) return fail(DC_ERR_INVALID, "bad shape B=%d V=%d", B, V);
+    // the kernel steps through logits and tokens in 32 bits
+    if (V >= 1 << 30 || ldt >= 1 << 30) return fail(DC_ERR_INVALID, "V and ldt must be below 2^30 (got %d, %d)", V, ldt);
     if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
     if (B == 0) return DC_OK;
     if (!logits || !out) return fail(DC_ERR_INVALID, "null pointer");
@@ -622,6 +624,7 @@ int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, c
 {
     clear_error();
     if (B < 0 || V <= 0 || ldl < V || ldt <= 0) return fail(DC_ERR_INVALID, "bad shape B=%d V=%d ldt=%d", B, V, ldt);
+    if (V >= 1 << 30) return fail(DC_ERR_INVALID, "V must be below 2^30 (got %d)", V);  // indices of 32 bits
     if (dtype != DC_F32 && dtype != DC_BF16) return fail(DC_ERR_INVALID, "bad dtype %d", dtype);
     if (B == 0) return DC_OK;
     if (!logits || !pos || !pos_out || !tokens) return fail(DC_ERR_INVALID, "null pointer");

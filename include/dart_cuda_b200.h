@@ -396,7 +396,8 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
  * 0: one for all rows; p < 0: no tokens yet), tokens [B, ldt], and per row
  * r = repetition[b] > 0, q = presence[b], f = frequency[b].  prompt_len NULL
  * stands for 0; each other array may be NULL (without effect).  Token ids
- * outside [0, V) are ignored.  A row whose mask allows nothing is all -inf. */
+ * outside [0, V) are ignored.  A row whose mask allows nothing is all -inf.
+ * V and ldt: below 2^30. */
 int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtype, int B, int V,
                        const int32_t *tokens, int ldt, const int32_t *pos, int pos_stride,
                        const int32_t *prompt_len, const float *repetition, const float *presence,
@@ -407,7 +408,7 @@ int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtyp
  * logits in `dtype`: tokens[b, p+1] = argmax (lowest index on ties), x[b,:] =
  * wte[token,:] + wpe[p+1,:] when x is non-NULL (wpe: at least ldt rows), and
  * pos_out[b] (may be pos) = p+1.  A row with p < 0 is left as it is; one with
- * p+1 >= ldt too, and sets status bit 0x40. */
+ * p+1 >= ldt too, and sets status bit 0x40.  V: below 2^30. */
 int dc_greedy_embed_rows(const void *logits, int ldl, int dtype, int B, int V, const float *wte,
                          const float *wpe, const int32_t *pos, int32_t *pos_out, int D,
                          int32_t *tokens, int ldt, float *x, void *stream);

@@ -132,3 +132,12 @@ def test_reference_packs_and_unpacks():
                 s = slice(32 * g, 32 * g + 32)
                 _, step, _ = ref.quantise_group(x[s])
                 assert np.abs(x[s].astype(np.float64) - y[s]).max() <= float(step) / 2
+
+
+@pytest.mark.parametrize("call,bad", [(controls, dict(V=2**30, ldl=2**30, ldo=2**30)),
+                                      (controls, dict(V=2**31 - 1, ldl=2**31 - 1, ldo=2**31 - 1)),
+                                      (controls, dict(ldt=2**30)), (controls, dict(ldt=2**31 - 1)),
+                                      (pick, dict(V=2**30, ldl=2**30)), (pick, dict(V=2**31 - 1, ldl=2**31 - 1))])
+def test_rows_past_the_kernels_indices_are_refused(L, call, bad):
+    """The kernels step through logits and tokens in 32 bits."""
+    assert call(L, **bad) == 1 and b"2^30" in L.dc_last_error()
