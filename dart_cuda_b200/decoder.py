@@ -712,7 +712,8 @@ class AftDecoder:
         sequence b's tokens are the first lens[b] + n_new of its row.
         ``controls`` act on the logits before each pick."""
         B, T0 = prompt.shape
-        if (T0 if lens is None else max(int(n) for n in lens)) + n_new > self.cfg.block_size:
+        lens = None if lens is None else [int(n) for n in lens]
+        if (T0 if lens is None else max(lens)) + n_new > self.cfg.block_size:
             raise ValueError("prompt + new tokens exceed the block size")
         self.prefill(prompt, lens=lens, cache_bits=cache_bits, n_new=n_new, page_size=page_size, controls=controls)
         steps = n_new - 1
