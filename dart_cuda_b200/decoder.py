@@ -584,7 +584,7 @@ class AftDecoder:
 
     def prefill(self, prompt: torch.Tensor, lens=None, cache_bits=32, n_new=None, page_size=16,
                 controls: LogitControls | None = None):
-        """Run the prompt [B, T0] (int32) through the batched forward, keep
+        """Run the prompt [B, T0] (int32, of any strides) through the batched forward, keep
         every layer's k/v history and pick the first new token (greedy).
 
         cache_bits=4 keeps the history in 4 bits, in pages of page_size
@@ -595,8 +595,14 @@ class AftDecoder:
         follows a shorter prompt in its row must be valid token ids and is
         otherwise ignored."""
         c, P = self.cfg, self.P
+        if prompt.dim() != 2 or prompt.dtype != torch.int32 or prompt.device != self.flat.device:
+            raise ValueError(f"the prompt must be [B, T0] int32 on {self.flat.device} (got {tuple(prompt.shape)} "
+                             f"{prompt.dtype} on {prompt.device})")
+        prompt = prompt.contiguous()  # the kernels read whole rows
         B, T0 = prompt.shape
         d, V, Tm = c.d_model, c.vocab, c.block_size
+        if T0 > Tm:
+            raise ValueError(f"prompt length {T0} exceeds block size {Tm}")
         if cache_bits not in (4, 32):
             raise ValueError(f"cache_bits must be 4 or 32 (got {cache_bits})")
         if lens is not None and cache_bits != 4:
