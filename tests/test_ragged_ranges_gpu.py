@@ -126,3 +126,59 @@ def test_aft_decode4_huge_bias(ops, H, hs, kind):
     got = check(h, 20)
     if kind == "nan":
         assert np.isnan(got).sum() == 32
+
+
+@pytest.mark.parametrize("H,hs,T,page,B,odd", [
+    (1, 64, 5000, 32, 1, 0), (1, 64, 4097, 16, 2, 1), (2, 128, 2000, 16, 3, 0), (8, 16, 1500, 8, 2, 1),
+    (1, 32, 3000, 64, 40, 0), (16, 16, 300, 8, 150, 1), (5, 64, 400, 128, 90, 0), (1, 128, 700, 256, 500, 0),
+    (2, 48, 2500, 64, 1, 0)])
+def test_aft_decode4_every_position_counts_once(ops, H, hs, T, page, B, odd):
+    """Keys of zero, biases of 0 or -inf and values that are whole numbers
+    0..15 make every weight 0 or 1 and both sums whole numbers below 2^24, so a
+    row is their quotient, rounded once (and halved by the gate): a position
+    that is lost or counted twice at a border of shares, blocks or pages is off
+    by 1 / (t + 1), far above that."""
+    rng = np.random.default_rng(T + B)
+    D, width = H * hs, -(-T // page)
+    v = rng.integers(0, 16, (B, T, D)).astype(np.float32)
+    v[..., ::32], v[..., 1::32] = 0, 15  # a group's low is 0, its step 1
+    keep = rng.random((H, T)) < 0.7
+    n_pages = B * width + 2
+    table = rng.permutation(n_pages)[: B * width].reshape(B, width).astype(np.int32)
+    pages = ops.kv4_pages(n_pages, page, D)
+    i = np.arange(T)
+    slots = cu((table[:, i // page] * page + i % page).reshape(-1).astype(np.int32))
+    flat = torch.from_numpy(v.reshape(B * T, D)).cuda()
+    ops.kv4_write(torch.zeros_like(flat), flat, slots, pages)
+    w = torch.zeros(H, T, T + odd, device="cuda")[:, :, odd:]
+    w.masked_fill_(cu(~keep)[:, None], float("-inf"))
+    on = np.repeat(keep, hs, 0).T  # [T, D]
+    ws, qkv, t_table = ops.aft_decode4_workspace(B, D), torch.zeros(B, 3 * D, device="cuda"), cu(table)
+    num = np.cumsum(np.where(on, v, 0), 1, dtype=np.float32)  # whole numbers: exact
+    den = np.cumsum(on, 0, dtype=np.float32)
+    assert num.max() < 2**24
+    rows = np.arange(B)
+    for k in range(25):
+        pos = rng.integers(0, T, B) if k % 3 else np.minimum(T - 1, T - 1 - k + rng.integers(0, 2, B))
+        if B > 2:
+            pos[rng.random(B) < 0.1] = rng.integers(0, 20)
+        qkv[:, 2 * D:] = cu(v[rows, pos])
+        got = ops.aft_decode4(qkv, w, pages, t_table, cu(pos.astype(np.int32)), ws).cpu().numpy()
+        n, d = num[rows, pos], den[pos]
+        want = 0.5 * np.where(d > 0, n / np.maximum(d, 1), 0)
+        assert np.all(np.abs(got - want) <= 2.0**-23 * want), (k, np.argwhere(np.abs(got - want) > 2.0**-23 * want)[:4])
+    assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("H,hs", SHAPES)
+@pytest.mark.parametrize("T", [200, 1100])
+def test_aft_decode4_keys_far_apart(ops, H, hs, T):
+    """Channels of a group whose keys lie hundreds apart are summed again,
+    whatever the slab's width, by a CTA alone or the last of several."""
+    rng = np.random.default_rng(H * hs + T)
+    D = H * hs
+    h = History(ops, rng, 2, H, hs, T, 8, "f32", [T - 1, T // 2])
+    kv = rng.standard_normal((2, T, 2 * D))
+    kv[..., :D] = 40 * kv[..., :D] + 150 * rng.standard_normal(D)
+    store(h, kv)
+    check(h, 900)
