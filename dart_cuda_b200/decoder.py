@@ -584,16 +584,18 @@ class AftDecoder:
 
     def prefill(self, prompt: torch.Tensor, lens=None, cache_bits=32, n_new=None, page_size=16,
                 controls: LogitControls | None = None):
-        """Run the prompt [B, T0] (int32, of any strides) through the batched forward, keep
-        every layer's k/v history and pick the first new token (greedy).
+        """Run the prompt [B, T0] (int32, of any strides) through the batched
+        forward, keep every layer's k/v history and pick the first new token
+        (greedy).
 
         cache_bits=4 keeps the history in 4 bits, in pages of page_size
         positions taken from a pool that holds the prompts and n_new tokens a
         sequence (by default, as many as fit the block size); the forward
         attends to the k and v that the history stands for, as the steps
         after it do.  lens (4 bits only): the prompts' lengths, 1..T0; what
-        follows a shorter prompt in its row must be valid token ids and is
-        otherwise ignored."""
+        follows a shorter prompt in its row must be valid token ids and tells
+        on the results by rounding only (the forward's AFT scales its operands
+        by their maxima over the row)."""
         c, P = self.cfg, self.P
         if prompt.dim() != 2 or prompt.dtype != torch.int32 or prompt.device != self.flat.device:
             raise ValueError(f"the prompt must be [B, T0] int32 on {self.flat.device} (got {tuple(prompt.shape)} "
