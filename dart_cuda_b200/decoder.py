@@ -95,10 +95,12 @@ class LogitControls:
     bias: torch.Tensor | None = None
     mask: torch.Tensor | None = None
 
-    def on(self, B, device, kept):
+    def on(self, B, device, kept=None):
         """Keyword arguments of ops.logits_controls for B sequences.  Copies
         lie in the tensors of ``kept`` (by name), the same for every call that
         fits them, so that a captured step reads the last call's."""
+        kept = {} if kept is None else kept
+
         def put(name, x, dtype=None, rows=None):
             if x is None:
                 return None
@@ -686,7 +688,9 @@ class AftDecoder:
         """Consume the token at position t = pos (its embedding is in s['x']),
         append its k/v to every layer's history, emit the token of t+1.  With
         a 4-bit history every sequence has a position of its own, and one
-        whose position is set to -1 is left out of further steps."""
+        whose position is set to -1 is left out of further steps.  One that
+        has filled the block size is to be left out: its further steps set
+        status bit 0x40 and may take pages from the others."""
         c, P = self.cfg, self.P
         s = self._dec
         x = s["x"]
