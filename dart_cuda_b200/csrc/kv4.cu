@@ -378,7 +378,9 @@ constexpr float kHuge = 0x1p24f;  // exponents of this size have no fraction in 
 // packed (a maximum a row instead: 113.0 instead of 110.3 us at 32 x <=8191).
 constexpr float kFar = 0x1p36f;
 constexpr float kAbsorbs = 1e30f;  // beside a finite bias of this size keys below 2^23 vanish, in 64 bits too
-constexpr int kItem = 10;   // what an item costs a CTA besides its blocks, in blocks
+// What an item costs a CTA besides its blocks, in blocks of 256 channels: this
+// and the shares' other constants were measured at that slab width.
+constexpr int kItem = 10;
 
 // 16 bytes, of which the first `bytes` (0 or 16) are read, the others zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes)
@@ -507,9 +509,9 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
 // What bounds it: a channel of a position costs one 2^x (8 cycles a warp and
 // scheduler) and about 7 other instructions that overlap with it imperfectly
 // (9.5 cycles alone), against 1.25 bytes of HBM, so 32 sequences of up to 8191
-// positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 111 us; the
+// positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 110 us; the
 // rest is what an item costs besides (merging, its first loads).  At 64
-// sequences of 256-511 positions, d = 512, these are most of the 14.5 us.  Steps
+// sequences of 256-511 positions, d = 512, these are most of the 14.6 us.  Steps
 // there: a lane per 8 channels 146 us (10.5 instructions a channel for
 // unpacking and bounds), 16 channels 183 us (too few registers), a group of 32
 // by four rows 141 us; codes through mixed-precision bf16 FMAs instead of byte
@@ -1073,7 +1075,7 @@ static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
     const dim3 grid((unsigned)decode_grid()), block(kThreads);
     constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
     // a bias for a group where heads allow it (32 sequences of up to 8191
-    // positions, hs = 128: 114 us, a bias for each 8 channels 145)
+    // positions, hs = 128: 110 us; hs = 120, d = 1920, a bias for each 8: 165)
     auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
     static SmemOnce once[2];
     const cudaError_t e = once[p.hs % 32 == 0].set(kernel, smem);

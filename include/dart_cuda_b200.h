@@ -374,7 +374,11 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
  * sequence with pos < 0 is left out and its Z row is zero; so is one with
  * pos >= c = min(Tmax, ldtab * page_size), which sets status bit 0x40, and one
  * whose bias row is -inf throughout.  c is below 2^20, and B * D/W * (c/16 +
- * 11) at most 2^30.  Sequences may share pages they only read.  workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
+ * 11) at most 2^30.  Sequences may share pages they only read.  Sums are held
+ * in fp32; an item that fp32 does not hold (keys hundreds apart or from 2^23
+ * on, a row of finite biases from about 2^24 on, values whose weighted sum
+ * overflows) is summed again in 64 bits, which takes longer.
+ * workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
  * zero-filled once before its first use (the kernel leaves its counters
  * zeroed), for this or any smaller B and D; calls that may overlap on the GPU
  * need one each. */
@@ -394,9 +398,10 @@ int dc_aft_decode4(const void *qkv, int ldq, int dtype, const float *w, int ldw,
  *                                   (ldm = 0: one for all rows)
  * with p = pos[b * pos_stride] the position the logits belong to (pos_stride
  * 0: one for all rows; p < 0: no tokens yet), tokens [B, ldt], and per row
- * r = repetition[b] > 0, q = presence[b], f = frequency[b].  prompt_len NULL
- * stands for 0; each other array may be NULL (without effect).  Token ids
- * outside [0, V) are ignored.  A row whose mask allows nothing is all -inf.
+ * r = repetition[b] > 0 (x / r is x times the rounded 1 / r), q = presence[b],
+ * f = frequency[b].  prompt_len NULL stands for 0; each other array may be
+ * NULL (without effect).  Token ids outside [0, V) are ignored.  A row whose
+ * mask allows nothing is all -inf.
  * V and ldt: below 2^30. */
 int dc_logits_controls(const void *logits, int ldl, void *out, int ldo, int dtype, int B, int V,
                        const int32_t *tokens, int ldt, const int32_t *pos, int pos_stride,
