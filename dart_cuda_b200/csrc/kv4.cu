@@ -402,9 +402,8 @@ __device__ __forceinline__ int row_blocks(const Decode &p, int t)
 
 __device__ __forceinline__ void join(float &m, float &num, float &den, float m2, float num2, float den2)
 {
-    const float mx = fmax_nan(m, m2);
-    if (mx == -INFINITY) return;
-    const float a = ex2(m - mx), c = ex2(m2 - mx);
+    const float mx = fmax_nan(m, m2), base = mx == -INFINITY ? 0.f : mx;  // masked so far: 0, or NaN of a value
+    const float a = ex2(m - base), c = ex2(m2 - base);
     num = num * a + num2 * c;
     den = den * a + den2 * c;
     m = mx;
@@ -431,8 +430,8 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
     }
     auto add = [](double &m, double &num, double &den, double m2, double num2, double den2) {
         const double mx = m2 > m || m2 != m2 ? m2 : m;  // NaN if either is
-        if (mx == -INFINITY) return;                    // masked so far
-        const float a = ex2((float)((m - mx) * 1.4426950408889634)), c = ex2((float)((m2 - mx) * 1.4426950408889634));
+        const double base = mx == -INFINITY ? 0. : mx;  // masked so far: 0, or NaN of a value
+        const float a = ex2((float)((m - base) * 1.4426950408889634)), c = ex2((float)((m2 - base) * 1.4426950408889634));
         num = num * a + num2 * c;
         den = den * a + den2 * c;
         m = mx;
@@ -1001,15 +1000,15 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                             float top = fm[k];
 #pragma unroll
                             for (int d = 0; d < N; ++d) top = fmax_nan(top, x[d][k][0]);
-                            if (top == -INFINITY) continue;  // masked so far
-                            const float a = ex2(fm[k] - top);
+                            const float base = top == -INFINITY ? 0.f : top;  // masked so far: 0, or NaN of a value
+                            const float a = ex2(fm[k] - base);
                             fn[k] *= a;
                             fd[k] *= a;
                             fm[k] = top;
 #pragma unroll
                             for (int d = 0; d < N; ++d) {
                                 if (g0 + d > j1) continue;
-                                const float c = ex2(x[d][k][0] - top);
+                                const float c = ex2(x[d][k][0] - base);
                                 fn[k] = fmaf(x[d][k][1], c, fn[k]);
                                 fd[k] = fmaf(x[d][k][2], c, fd[k]);
                             }

@@ -182,3 +182,23 @@ def test_aft_decode4_keys_far_apart(ops, H, hs, T):
     kv[..., :D] = 40 * kv[..., :D] + 150 * rng.standard_normal(D)
     store(h, kv)
     check(h, 900)
+
+
+@pytest.mark.parametrize("H,hs", SHAPES)
+@pytest.mark.parametrize("T", [90, 700])
+def test_aft_decode4_not_finite_under_masks(ops, H, hs, T):
+    """A value that is not finite reaches its group's outputs from a position
+    that -inf masks too (0 * NaN), wherever it lies, and no others; a sequence
+    whose positions are all masked stays zero."""
+    rng = np.random.default_rng(H * hs + T)
+    D = H * hs
+    for at in (0, 1, 17, T - 2):
+        w = (0.5 * rng.standard_normal((H, T, T))).astype(np.float32)
+        w[:, :, : T // 2] = -np.inf
+        w[:, T - 1, at] = -np.inf
+        kv = rng.standard_normal((2, T, 2 * D))
+        kv[0, at, D + 5] = np.nan
+        h = History(ops, rng, 2, H, hs, T, 8, "f32", [T - 1, T // 2 - 1], w=w)
+        store(h, kv)
+        got = check(h, 20)
+        assert np.flatnonzero(np.isnan(got[0])).tolist() == list(range(32)) and not got[1].any()
