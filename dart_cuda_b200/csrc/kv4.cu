@@ -491,7 +491,8 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
 // have lost terms to underflow (a scale below 2^-126 becomes 0, and what it
 // scales is at most 2^16 a position), and values may be so large (up to 1e37
 // times a weight of up to 2^16) that num overflows, which leaves it infinite or
-// NaN beside a finite den: such an item is then summed again, in 64 bits and
+// NaN beside a finite den, or so small (below 2^-28) that num lies below 2^-90
+// and may have lost terms too: such an item is then summed again, in 64 bits and
 // with a running maximum per channel.  So are those whose exponents fp32 does
 // not hold: references from 2^24 on (a row masked throughout by -1e9) and keys
 // from 2^23 on, which a bias of their size may cancel.  Beside smaller keys a
@@ -1027,7 +1028,8 @@ __global__ void __launch_bounds__(kThreads, kResident) decode_kernel(const __gri
                     if (tid + k * kThreads >= W || fm[k] == -INFINITY) continue;
                     const float far = fabsf(fm[k]);
                     lost |= (far >= kHuge && far < 0.5f * kAbsorbs) || far == INFINITY || fd[k] < 0x1p-64f ||
-                            (fd[k] < INFINITY && !(fabsf(fn[k]) < INFINITY));
+                            (fd[k] < INFINITY && !(fabsf(fn[k]) < INFINITY)) ||
+                            (fabsf(fn[k]) < 0x1p-90f && (fn[k] != 0.f || fd[k] < 0x1p-32f));
                 }
                 if (__syncthreads_or(lost)) {
                     const float *mean = resum<W>(p, b, slab, t, part(0));

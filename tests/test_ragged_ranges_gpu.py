@@ -202,3 +202,19 @@ def test_aft_decode4_not_finite_under_masks(ops, H, hs, T):
         store(h, kv)
         got = check(h, 20)
         assert np.flatnonzero(np.isnan(got[0])).tolist() == list(range(32)) and not got[1].any()
+
+
+@pytest.mark.parametrize("H,hs", SHAPES)
+@pytest.mark.parametrize("size", [1e-10, 1e-20, 1e-28, 1e-33])
+def test_aft_decode4_small_values(ops, H, hs, size):
+    """Values whose products with small weights fall below fp32's range:
+    channels up to 40 nats below their group's reference."""
+    rng = np.random.default_rng(H * hs)
+    D, T = H * hs, 150
+    h = History(ops, rng, 2, H, hs, T, 8, "f32", [T - 1, 60])
+    kv = rng.standard_normal((2, T, 2 * D))
+    kv[..., :D] += rng.uniform(-20, 20, D)
+    kv[..., D:] *= size
+    store(h, kv)
+    h.qkv[:, 2 * D:] *= size
+    check(h, 40)
