@@ -511,7 +511,7 @@ __device__ __noinline__ const float *resum(const Decode &p, int b, int slab, int
 // (9.5 cycles alone), against 1.25 bytes of HBM, so 32 sequences of up to 8191
 // positions, d = 2048 (345 MB, 53 us of HBM, 59 us of 2^x) take 110 us; the
 // rest is what an item costs besides (merging, its first loads).  At 64
-// sequences of 256-511 positions, d = 512, these are most of the 14.6 us.  Steps
+// sequences of 256-511 positions, d = 512, these are most of the 14.3 us.  Steps
 // there: a lane per 8 channels 146 us (10.5 instructions a channel for
 // unpacking and bounds), 16 channels 183 us (too few registers), a group of 32
 // by four rows 141 us; codes through mixed-precision bf16 FMAs instead of byte
@@ -1076,7 +1076,7 @@ static cudaError_t launch_slab(const Decode &p, cudaStream_t st)
     const dim3 grid((unsigned)decode_grid()), block(kThreads);
     constexpr int smem = kWarps * kStages * (256 / W) * kRows * (W * 5 / 4);
     // a bias for a group where heads allow it (32 sequences of up to 8191
-    // positions, hs = 128: 110 us; hs = 120, d = 1920, a bias for each 8: 165)
+    // positions, hs = 128: 110 us; hs = 120, d = 1920, a bias for each 8: 163)
     auto kernel = p.hs % 32 == 0 ? decode_kernel<T, W, 1> : decode_kernel<T, W, 4>;
     static SmemOnce once[2];
     const cudaError_t e = once[p.hs % 32 == 0].set(kernel, smem);

@@ -376,8 +376,9 @@ int dc_kv4_write(const void *k, const void *v, int ld, int dtype, const int32_t 
  * whose bias row is -inf throughout.  c is below 2^20, and B * D/W * (c/16 +
  * 11) at most 2^30.  Sequences may share pages they only read.  Sums are held
  * in fp32; an item that fp32 does not hold (keys hundreds apart or from 2^23
- * on, a row of finite biases from about 2^24 on, values whose weighted sum
- * overflows) is summed again in 64 bits, which takes longer.
+ * on, a row of finite biases from about 2^24 on, values above 1e33 or below
+ * 1e-28 whose weighted sums leave its range) is summed again in 64 bits, which
+ * takes longer.
  * workspace: dc_aft_decode4_workspace_size bytes, 16-byte aligned,
  * zero-filled once before its first use (the kernel leaves its counters
  * zeroed), for this or any smaller B and D; calls that may overlap on the GPU
